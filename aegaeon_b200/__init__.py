@@ -13,9 +13,10 @@ import importlib
 __version__ = "0.1.0"
 
 _SUBMODULES = ("build", "layout", "ops", "step", "synth")
-_OPS_EXPORTS = ("DecodePlan", "copy_blocks", "decode_layer", "decode_layer_flash", "flash_attn_decode",
-                "paged_attention_decode", "read_device_errors", "reshape_and_cache", "reshape_and_cache_flash",
-                "swap", "swap_sm")
+_OPS_EXPORTS = ("DecodePlan", "compact_blocks", "copy_blocks", "decode_layer", "decode_layer_flash",
+                "flash_attn_decode", "fork_blocks", "free_blocks", "gather_cache_int4", "paged_attention_decode",
+                "read_device_errors", "reshape_and_cache", "reshape_and_cache_flash", "reshape_and_cache_int4",
+                "rotary_multi_axis", "swap", "swap_sm")
 
 __all__ = list(_SUBMODULES) + list(_OPS_EXPORTS)
 

@@ -24,6 +24,8 @@ AEG_DEVERR_SLOT_RANGE = 0x2
 AEG_DEVERR_SEQ_LEN_RANGE = 0x4
 AEG_DEVERR_WAIT_TIMEOUT = 0x8
 AEG_DEVERR_PLAN_MISMATCH = 0x10
+AEG_DEVERR_POOL_ENTRY = 0x20
+AEG_DEVERR_POOL_EMPTY = 0x40
 
 AEG_DECODE_PREFETCH = 0x1
 AEG_DECODE_PREFETCH_AFTER_DECODE_WRITE = 0x2
@@ -72,6 +74,20 @@ SIGNATURES = {
     "aeg_paged_attn_decode_noalloc": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64,
                                              _c_void_p, _i32, _c_void_p, _i32, _i32, _i32, _i32, ctypes.c_float,
                                              _i32, _c_void_p]),
+    "aeg_reshape_and_cache_int4": (_i32, [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64,
+                                          _i32, _i32, _i32, _c_void_p]),
+    "aeg_gather_cache_int4": (_i32, [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i32,
+                                     _i32, _i32, _c_void_p]),
+    "aeg_rotary_multi_axis": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,
+                                     _i64, _i32, _c_void_p, _c_void_p, _i32, ctypes.c_float, _i64, _i32, _i32, _i32,
+                                     _i32, _c_void_p]),
+    "aeg_fork_blocks_workspace_size": (_sz, [_i64]),
+    "aeg_fork_blocks": (_i32, [_c_void_p, _sz, _i64, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _c_void_p,
+                               _c_void_p, _i64, _c_void_p, _c_void_p, _sz, _c_void_p]),
+    "aeg_free_blocks": (_i32, [_i64, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _c_void_p, _i64, _c_void_p]),
+    "aeg_compact_blocks_workspace_size": (_sz, [_i64]),
+    "aeg_compact_blocks": (_i32, [_c_void_p, _sz, _i64, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _c_void_p,
+                                  _c_void_p, _c_void_p, _c_void_p, _c_void_p, _sz, _c_void_p]),
 }
 
 

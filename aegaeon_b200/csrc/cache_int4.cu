@@ -1,0 +1,263 @@
+// The 4-bit KV cache's write (reshape_and_cache_int4) and read-back (gather_cache_int4).
+//
+// The write is reshape_and_cache (cache_write.cu) with the rows rounded to 4 bits: slot s is row
+// s % 16 of the tiles of block s / 16, a slot < 0 is padding. Format and layout: int4_tile.cuh.
+// Both are bound by memory: 512 bytes of keys and values a (token, head) on one side, 144 bytes of
+// codes and pairs on the other. One warp moves one (token, head): lanes 0..15 its key, 16..31 its
+// value, 8 dims a lane (one 16-byte vector), 8 lanes a 64-dim group, so that a group's range is
+// three shuffles away and a lane's codes are exactly one key word or two value halves. A warp takes
+// kItems of them at a time, all loads before the first use.
+#include "int4_tile.cuh"
+
+#include <algorithm>
+
+namespace aeg {
+namespace {
+
+__device__ unsigned int g_deverr_int4 = 0;
+
+constexpr int kThreads = 128;
+constexpr int kWarpsPerCta = kThreads / 32;
+
+// A lane's 8 elements of a row: one 16-byte vector, or 8 loads where rows are not 16-byte aligned.
+template <bool kVec>
+__device__ __forceinline__ uint4 load8(const uint16_t* p) {
+  if constexpr (kVec) {
+    return *reinterpret_cast<const uint4*>(p);
+  } else {
+    return make_uint4(p[0] | (uint32_t(p[1]) << 16), p[2] | (uint32_t(p[3]) << 16), p[4] | (uint32_t(p[5]) << 16),
+                      p[6] | (uint32_t(p[7]) << 16));
+  }
+}
+
+template <bool kVec>
+__device__ __forceinline__ void store8(uint16_t* p, const uint4& v) {
+  if constexpr (kVec) {
+    *reinterpret_cast<uint4*>(p) = v;
+  } else {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      p[2 * i] = static_cast<uint16_t>(w[i]);
+      p[2 * i + 1] = static_cast<uint16_t>(w[i] >> 16);
+    }
+  }
+}
+
+struct Rows {
+  uint16_t* key;
+  uint16_t* value;
+  int64_t key_stride;    // elements between tokens
+  int64_t value_stride;
+  uint8_t* cache;        // the layer's first tile
+  int64_t block_stride;  // bytes between blocks
+  const int64_t* slots;
+  int64_t num_slots;
+  int64_t items;  // tokens * heads
+  int heads;
+};
+
+template <typename T, bool kVec, int kItems>
+__global__ void __launch_bounds__(kThreads) write_int4_kernel(const Rows p) {
+  pdl_launch_dependents();
+  pdl_wait_primary();
+  const int lane = threadIdx.x & 31, l = lane & 15;
+  const bool is_key = lane < 16;
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarpsPerCta;
+  const int64_t warp = static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5);
+  const uint16_t* rows = is_key ? p.key : p.value;
+  const int64_t stride = is_key ? p.key_stride : p.value_stride;
+  for (int64_t i0 = warp * kItems; i0 < p.items; i0 += warps * kItems) {
+    uint4 v[kItems];
+    int64_t slot[kItems];
+    int head[kItems];
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const int64_t i = min(i0 + k, p.items - 1);
+      const int64_t t = i / p.heads;
+      head[k] = static_cast<int>(i - t * p.heads);
+      slot[k] = p.slots[t];
+      v[k] = load8<kVec>(rows + t * stride + head[k] * kInt4Dim + 8 * l);
+      if (i0 + k >= p.items) slot[k] = -1;
+    }
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      float x[8];
+      const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const float2 f = unpack2<T>(w[n]);
+        x[2 * n] = f.x;
+        x[2 * n + 1] = f.y;
+      }
+      uint32_t word, pair;
+      int4_quantise<T>(x, word, pair);
+      if (slot[k] >= p.num_slots) {
+        if (lane == 0) atomicOr(&g_deverr_int4, AEG_DEVERR_SLOT_RANGE);
+      } else if (slot[k] >= 0) {
+        const int t = static_cast<int>(slot[k] & 15);
+        uint8_t* tile = p.cache + (slot[k] >> 4) * p.block_stride + static_cast<int64_t>(head[k]) * kInt4TileBytes;
+        if (is_key) {
+          *reinterpret_cast<uint32_t*>(tile + int4_key_word(t, l)) = word;
+        } else {
+          uint16_t* half = reinterpret_cast<uint16_t*>(tile + int4_value_half(t, l));
+          half[0] = static_cast<uint16_t>(word);
+          half[2] = static_cast<uint16_t>(word >> 16);
+        }
+        if ((l & 7) == 0)
+          *reinterpret_cast<uint32_t*>(tile + (is_key ? kInt4KeyPairs : kInt4ValuePairs) + t * 8 + (l >> 3) * 4) = pair;
+      }
+    }
+  }
+}
+
+template <typename T, bool kVec, int kItems>
+__global__ void __launch_bounds__(kThreads) gather_int4_kernel(const Rows p) {
+  pdl_launch_dependents();
+  pdl_wait_primary();
+  const int lane = threadIdx.x & 31, l = lane & 15;
+  const bool is_key = lane < 16;
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarpsPerCta;
+  const int64_t warp = static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5);
+  uint16_t* rows = is_key ? p.key : p.value;
+  const int64_t stride = is_key ? p.key_stride : p.value_stride;
+  for (int64_t i0 = warp * kItems; i0 < p.items; i0 += warps * kItems) {
+    uint32_t word[kItems], pair[kItems];
+    int64_t token[kItems], slot[kItems];
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      token[k] = min(i0 + k, p.items - 1) / p.heads;
+      slot[k] = p.slots[token[k]];
+    }
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      word[k] = 0;
+      pair[k] = 0;  // scale 0, minimum 0: zeros
+      if (slot[k] >= 0 && slot[k] < p.num_slots) {
+        const int head = static_cast<int>(min(i0 + k, p.items - 1) - token[k] * p.heads);
+        const int t = static_cast<int>(slot[k] & 15);
+        const uint8_t* tile = p.cache + (slot[k] >> 4) * p.block_stride + static_cast<int64_t>(head) * kInt4TileBytes;
+        if (is_key) {
+          word[k] = *reinterpret_cast<const uint32_t*>(tile + int4_key_word(t, l));
+        } else {
+          const uint16_t* half = reinterpret_cast<const uint16_t*>(tile + int4_value_half(t, l));
+          word[k] = half[0] | (uint32_t(half[2]) << 16);
+        }
+        pair[k] = *reinterpret_cast<const uint32_t*>(tile + (is_key ? kInt4KeyPairs : kInt4ValuePairs) + t * 8 + (l >> 3) * 4);
+      } else if (slot[k] >= p.num_slots && lane == 0) {
+        atomicOr(&g_deverr_int4, AEG_DEVERR_SLOT_RANGE);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      if (i0 + k >= p.items) break;
+      const float2 sm = unpack2<T>(pair[k]);
+      // One rounding to fp32 (code * scale alone is exact), one to the type.
+      auto value = [&](int n) { return fmaf(static_cast<float>((word[k] >> (4 * n)) & 15u), sm.x, sm.y); };
+      const uint4 out = make_uint4(pack2<T>(value(0), value(1)), pack2<T>(value(2), value(3)),
+                                   pack2<T>(value(4), value(5)), pack2<T>(value(6), value(7)));
+      const int64_t head = i0 + k - token[k] * p.heads;
+      store8<kVec>(rows + token[k] * stride + head * kInt4Dim + 8 * l, out);
+    }
+  }
+}
+
+// Checks shared by both directions; fills `p`.
+int prepare(const char* what, Rows& p, const void* key, const void* value, int64_t key_stride, int64_t value_stride,
+            const void* cache, int64_t block_stride, int64_t num_blocks, const int64_t* slot_mapping, int64_t T, int Hkv,
+            int D, int dtype) {
+  AEG_CHECK_ARG(T >= 0 && T <= 0x7fffffffLL, "%s: token count %lld out of range", what, (long long)T);
+  AEG_CHECK_ARG(Hkv > 0 && D > 0, "%s: Hkv and D must be positive", what);
+  if (D != kInt4Dim) return set_error(AEG_ERR_UNSUPPORTED, "%s: head_dim %d not supported (only 128)", what, D);
+  AEG_CHECK_ARG(dtype == AEG_DTYPE_FP16 || dtype == AEG_DTYPE_BF16, "%s: dtype %d is not fp16/bf16", what, dtype);
+  AEG_CHECK_ARG(num_blocks >= 0 && num_blocks <= 0x7fffffffLL, "%s: num_blocks %lld out of range", what, (long long)num_blocks);
+  if (T == 0) return AEG_OK;
+  AEG_CHECK_ARG(key && value && cache && slot_mapping, "%s: null pointer", what);
+  const int64_t row = int64_t(Hkv) * D;
+  AEG_CHECK_ARG(key_stride >= row && value_stride >= row, "%s: token stride smaller than Hkv*D", what);
+  AEG_CHECK_ARG(block_stride >= int64_t(Hkv) * kInt4TileElems && block_stride % 8 == 0,
+                "%s: block stride must be a multiple of 8 elements and >= Hkv*1152", what);
+  AEG_CHECK_ARG(aligned(cache, 16), "%s: the cache must be 16-byte aligned", what);
+  AEG_CHECK_ARG(aligned(key, 2) && aligned(value, 2) && aligned(slot_mapping, 8), "%s: misaligned pointer", what);
+  p.key = static_cast<uint16_t*>(const_cast<void*>(key));
+  p.value = static_cast<uint16_t*>(const_cast<void*>(value));
+  p.key_stride = key_stride;
+  p.value_stride = value_stride;
+  p.cache = static_cast<uint8_t*>(const_cast<void*>(cache));
+  p.block_stride = 2 * block_stride;
+  p.slots = slot_mapping;
+  p.num_slots = num_blocks * 16;
+  p.items = T * Hkv;
+  p.heads = Hkv;
+  return AEG_OK;
+}
+
+using Kernel = void (*)(const Rows);
+
+template <typename T, int kItems>
+Kernel pick(bool write, bool vec) {
+  if (write) return vec ? write_int4_kernel<T, true, kItems> : write_int4_kernel<T, false, kItems>;
+  return vec ? gather_int4_kernel<T, true, kItems> : gather_int4_kernel<T, false, kItems>;
+}
+
+constexpr int kManyItems = 4;
+
+int launch(const char* what, bool write, const Rows& p, int dtype, cudaStream_t stream) {
+  const bool vec = aligned(p.key, 16) && aligned(p.value, 16) && p.key_stride % 8 == 0 && p.value_stride % 8 == 0;
+  // Several items a warp only once every SM's warps have one.
+  const int64_t resident = int64_t(num_sms()) * 16 * kWarpsPerCta;
+  const bool many = p.items >= resident;
+  const Kernel k = dtype == AEG_DTYPE_BF16
+                       ? (many ? pick<__nv_bfloat16, kManyItems>(write, vec) : pick<__nv_bfloat16, 1>(write, vec))
+                       : (many ? pick<__half, kManyItems>(write, vec) : pick<__half, 1>(write, vec));
+  const int64_t per_cta = int64_t(kWarpsPerCta) * (many ? kManyItems : 1);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>((p.items + per_cta - 1) / per_cta, int64_t(num_sms()) * 16)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  AEG_CHECK_CUDA(cudaLaunchKernelEx(&cfg, k, p));
+  AEG_CHECK_LAUNCH(what);
+  return AEG_OK;
+}
+
+}  // namespace
+
+uint32_t deverr_read_and_clear_int4(cudaStream_t s, cudaError_t* err) {
+  uint32_t v = 0, zero = 0;
+  *err = cudaMemcpyFromSymbolAsync(&v, g_deverr_int4, sizeof(v), 0, cudaMemcpyDeviceToHost, s);
+  if (*err == cudaSuccess) *err = cudaStreamSynchronize(s);
+  if (*err == cudaSuccess) *err = cudaMemcpyToSymbolAsync(g_deverr_int4, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s);
+  if (*err == cudaSuccess) *err = cudaStreamSynchronize(s);
+  return v;
+}
+
+}  // namespace aeg
+
+extern "C" {
+
+int aeg_reshape_and_cache_int4(const void* key, const void* value, int64_t key_stride, int64_t value_stride,
+                               void* kv_cache, int64_t block_stride, int64_t num_blocks, const int64_t* slot_mapping,
+                               int64_t T, int Hkv, int D, int dtype, void* stream) {
+  aeg::Rows p{};
+  const int st = aeg::prepare("reshape_and_cache_int4", p, key, value, key_stride, value_stride, kv_cache, block_stride,
+                              num_blocks, slot_mapping, T, Hkv, D, dtype);
+  if (st != AEG_OK || T == 0) return st;
+  return aeg::launch("reshape_and_cache_int4", true, p, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int aeg_gather_cache_int4(void* key, void* value, int64_t key_stride, int64_t value_stride, const void* kv_cache,
+                          int64_t block_stride, int64_t num_blocks, const int64_t* slot_mapping, int64_t T, int Hkv,
+                          int D, int dtype, void* stream) {
+  aeg::Rows p{};
+  const int st = aeg::prepare("gather_cache_int4", p, key, value, key_stride, value_stride, kv_cache, block_stride,
+                              num_blocks, slot_mapping, T, Hkv, D, dtype);
+  if (st != AEG_OK || T == 0) return st;
+  return aeg::launch("gather_cache_int4", false, p, dtype, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,123 @@
+// The 4-bit KV-cache tile: 16 tokens of one (block, layer, KV head), 128 dims, keys and values.
+//
+// An element stands for code * scale + minimum, with one (scale, minimum) pair of the model's
+// 16-bit type per token and 64-dim group:
+//   minimum = min of the group (exact: it is one of the inputs)
+//   scale   = (max - min) / 15, rounded once to the type (nearest, ties to even)
+//   code    = (x - minimum) / scale, rounded to the nearest whole number (ties to even), 0..15
+// A group whose max - min is not finite (a NaN, an infinity, or a spread beyond fp32) has NaN for
+// both, so that it reads back as NaN instead of as plausible numbers; scale 0 has code 0.
+//
+// Bytes of a tile (2304 = 18 x 128, contiguous, so that one bulk copy fetches it):
+//   [0, 1024)     key codes: token t at t * 64, in four 16-byte chunks; chunk c, word w holds dims
+//                 32 w + 8 c + n at bits 4 n. Lane (row g, column c) of an MMA fragment finds all
+//                 of its codes of token g in one 16-byte load, and words 0, 1 / 2, 3 belong to
+//                 groups 0 / 1.
+//   [1024, 2048)  value codes: tokens 2 p and 2 p + 1 at p * 128, in eight 16-byte chunks; chunk g,
+//                 word w holds dims 64 (w / 2) + 8 g + 4 (w % 2) + n of token 2 p at bits 4 n and of
+//                 token 2 p + 1 at bits 16 + 4 n. A byte belongs to one token, so writing a token
+//                 touches no other one's bytes.
+//   [2048, 2176)  key pairs: (scale, minimum) of token t, group g at t * 8 + g * 4
+//   [2176, 2304)  value pairs, likewise
+#pragma once
+
+#include "aeg_common.cuh"
+
+namespace aeg {
+
+constexpr int kInt4Dim = 128;
+constexpr int kInt4Group = 64;
+constexpr int kInt4TileBytes = 2304;
+constexpr int kInt4TileElems = kInt4TileBytes / 2;
+constexpr int kInt4ValueCodes = 1024;
+constexpr int kInt4KeyPairs = 2048;
+constexpr int kInt4ValuePairs = 2176;
+
+// Byte offset of the key word that holds dims 8 l .. 8 l + 7 (l = 0..15) of token t.
+__host__ __device__ __forceinline__ int int4_key_word(int t, int l) { return t * 64 + (l & 3) * 16 + (l >> 2) * 4; }
+// Byte offset of the 16-bit half that holds value dims 8 l .. 8 l + 3 of token t; the half of dims
+// 8 l + 4 .. 8 l + 7 lies 4 bytes further on.
+__host__ __device__ __forceinline__ int int4_value_half(int t, int l) {
+  return kInt4ValueCodes + (t >> 1) * 128 + (l & 7) * 16 + (l >> 3) * 8 + (t & 1) * 2;
+}
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// The 16 bits of `v` rounded once to T: to 24 bits with the lost part kept as a sticky last bit
+// (round to odd), from which the rounding to T's 8 or 11 bits comes out as if made from `v`.
+template <typename T>
+__device__ __forceinline__ T round_once(double v) {
+  const float f = __double2float_rz(v);
+  uint32_t bits = __float_as_uint(f);
+  if (static_cast<double>(f) != v) bits |= 1u;
+  return from_float<T>(__uint_as_float(bits));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t bits16(T v) {
+  return static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&v));
+}
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v);
+template <>
+__device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Codes of a lane's 8 dims and its group's pair. The 8 lanes of a group are consecutive and call
+// this together. `word` holds dim n's code at bits 4 n; the pair is scale | minimum << 16.
+//
+// Codes are decided in fp32 without a rounding error in the decision: c = rint(d / s) by a
+// reciprocal is right or next to it, c * s has at most 15 bits, and d - c * s comes out of one FMA
+// exactly, as |d - c s| <= s and d <= 16 s or so. Only where it is exactly half a scale does the
+// rounding error e of d = x - minimum itself count.
+template <typename T>
+__device__ __forceinline__ void int4_quantise(const float (&x)[8], uint32_t& word, uint32_t& pair) {
+  float lo = x[0], hi = x[0];
+#pragma unroll
+  for (int n = 1; n < 8; ++n) {
+    lo = min_nan(lo, x[n]);
+    hi = max_nan(hi, x[n]);
+  }
+#pragma unroll
+  for (int off = 1; off < 8; off <<= 1) {
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+  }
+  const bool ok = isfinite(hi - lo);
+  const T scale = round_once<T>(ok ? (static_cast<double>(hi) - static_cast<double>(lo)) / 15.0 : 0.0);
+  float s = to_float<T>(scale);
+  word = 0;
+  pair = ok ? (bits16(scale) | (bits16(from_float<T>(lo)) << 16)) : 0x7fff7fffu;
+  if (!ok || s == 0.f) return;
+  // Far below 1, both sides are scaled up exactly so that the reciprocal stays finite.
+  const float up = s < 1e-30f ? 18446744073709551616.f : 1.f;
+  s *= up;
+  const float r = __frcp_rn(s), half = 0.5f * s;
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    const float d0 = x[n] - lo, d = d0 * up;
+    float c = fminf(rintf(d * r), 15.f);
+    const float rest = fmaf(-c, s, d);
+    if (fabsf(rest) >= half) {
+      const float back = d0 - x[n];
+      const float e = (x[n] - (d0 - back)) + (-lo - back);  // x - lo = d0 + e
+      const bool odd = (static_cast<int>(c) & 1) != 0;
+      if (rest > half || (rest == half && (e > 0.f || (e == 0.f && odd)))) c = fminf(c + 1.f, 15.f);
+      else if (rest < -half || (rest == -half && (e < 0.f || (e == 0.f && odd)))) c -= 1.f;
+    }
+    word |= static_cast<uint32_t>(static_cast<int>(c)) << (4 * n);
+  }
+}
+
+}  // namespace aeg

@@ -27,6 +27,21 @@ def kv_block_shape(num_layers: int, num_kv_heads: int, head_dim: int) -> tuple[i
     return (num_layers, 2, BLOCK_SIZE, num_kv_heads, head_dim)
 
 
+# 16-bit elements of one tile of a 4-bit cache: 16 tokens of one (block, layer, KV head) with 128
+# dims, i.e. 1024 bytes of key codes, 1024 of value codes and a (scale, minimum) pair per token and
+# 64-dim group for either (include/aegaeon_b200.h).
+INT4_TILE = 1152
+
+
+def int4_block_shape(num_layers: int, num_kv_heads: int, head_dim: int = 128) -> tuple[int, ...]:
+    """Per-block shape ``(L, Hkv, 1152)`` of a 4-bit KV cache, in elements of the model's 16-bit type:
+    ``torch.zeros((N, *int4_block_shape(L, Hkv)), dtype=torch.bfloat16, device="cuda")``. The elements
+    are containers (codes and pairs), not values; ``ops.gather_cache_int4`` reads them back."""
+    if head_dim != 128:
+        raise NotImplementedError(f"4-bit caches support head_dim 128, not {head_dim}")
+    return (num_layers, num_kv_heads, INT4_TILE)
+
+
 def kv_cache_run_view(kv_cache: torch.Tensor) -> torch.Tensor:
     """The ``(L, 2, N, 16, Hkv, D)`` view the model layers index by ``[layer][0|1]``."""
     if kv_cache.dim() != 6:

@@ -14,15 +14,16 @@ or PyTorch fallback: the work always runs in the CUDA library.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
-from typing import Sequence
+from typing import NamedTuple, Sequence
 
 import numpy as np
 import torch
 
 from . import _native
 from ._native import AEG_DECODE_PREFETCH, AEG_DECODE_PREFETCH_AFTER_DECODE_WRITE, check, lib
-from .layout import BLOCK_SIZE, block_bytes
+from .layout import BLOCK_SIZE, INT4_TILE, block_bytes
 
 _DTYPES = {torch.float16: _native.AEG_DTYPE_FP16, torch.bfloat16: _native.AEG_DTYPE_BF16}
 
@@ -534,6 +535,274 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Te
     """Writes the new tokens' K/V of ``layer`` into Aegaeon's ``(N, L, 2, 16, Hkv, D)`` cache."""
     kc, vc = _layer_views(kv_cache, layer)
     reshape_and_cache_flash(key, value, kc, vc, slot_mapping)
+
+
+# --------------------------------------------------------------------------------------------
+# 4-bit KV cache (layout.int4_block_shape): write and read-back
+
+
+def _int4_layer(kv_cache: torch.Tensor, layer: int, heads: int | None = None) -> int:
+    """Checks a 4-bit cache (and its KV head count) and returns the address of ``layer``'s first tile."""
+    _require_cuda(kv_cache, "kv_cache")
+    if kv_cache.dim() != 4 or kv_cache.size(3) != INT4_TILE or kv_cache.dtype not in _DTYPES:
+        raise ValueError(f"kv_cache must be a 4-bit cache (N, L, Hkv, {INT4_TILE}) of fp16 or bf16, got "
+                         f"{tuple(kv_cache.shape)} of {kv_cache.dtype}")
+    if not kv_cache.is_contiguous():
+        raise ValueError("kv_cache must be contiguous")
+    if heads is not None and kv_cache.size(2) != heads:
+        raise ValueError(f"kv_cache holds {kv_cache.size(2)} KV heads, not {heads}")
+    if not 0 <= layer < kv_cache.size(1):
+        raise ValueError(f"layer {layer} outside [0, {kv_cache.size(1)})")
+    return kv_cache.data_ptr() + layer * kv_cache.size(2) * INT4_TILE * 2
+
+
+def _int4_rows(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    for name, t in (("key", key), ("value", value)):
+        _require_cuda(t, name)
+        if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.size(2):
+            raise ValueError(f"{name} must be [T, Hkv, D] with contiguous heads")
+        if t.dtype != kv_cache.dtype:
+            raise ValueError(f"{name} dtype {t.dtype} differs from cache dtype {kv_cache.dtype}")
+    if key.shape != value.shape:
+        raise ValueError("key and value must have the same shape")
+    _require_cuda(slot_mapping, "slot_mapping")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1 or slot_mapping.numel() != key.size(0):
+        raise ValueError("slot_mapping must be int64 [T]")
+    _same_device(kv_cache.device, key=key, value=value, slot_mapping=slot_mapping)
+
+
+def reshape_and_cache_int4(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, layer: int,
+                           slot_mapping: torch.Tensor) -> None:
+    """Rounds the new tokens' K/V of ``layer`` to 4 bits and writes them into a 4-bit cache.
+
+    ``key``/``value`` ``[T, Hkv, 128]`` of the cache's dtype (any token stride), ``kv_cache``
+    ``(N, L, Hkv, 1152)`` (``layout.int4_block_shape``), ``slot_mapping`` int64 ``[T]``: slot s is row
+    s % 16 of block s // 16, s < 0 is padding. Every 64-dim group of a row is held as ``code * scale +
+    minimum`` with a 4-bit code; a group with a NaN or an infinity reads back as NaN. The slots of one
+    call must be distinct.
+    """
+    base = _int4_layer(kv_cache, layer, key.size(1) if isinstance(key, torch.Tensor) and key.dim() == 3 else None)
+    _int4_rows(key, value, kv_cache, slot_mapping)
+    slot_mapping = slot_mapping.contiguous()
+    dev = kv_cache.device
+    with torch.cuda.device(dev):
+        st = lib.aeg_reshape_and_cache_int4(key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0), base,
+                                            kv_cache.stride(0), kv_cache.size(0), slot_mapping.data_ptr(), key.size(0),
+                                            key.size(1), key.size(2), _DTYPES[kv_cache.dtype], _stream(dev))
+    check(st, "reshape_and_cache_int4")
+
+
+def gather_cache_int4(kv_cache: torch.Tensor, layer: int, slot_mapping: torch.Tensor, key: torch.Tensor | None = None,
+                      value: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values ``[T, Hkv, 128]`` held at ``slot_mapping`` (int64 ``[T]``) of ``layer``, in the
+    cache's dtype: what a prompt that continues a cached prefix attends to, or what a 16-bit cache
+    takes over. Slots < 0 give zero rows. ``key``/``value`` receive the result when given."""
+    base = _int4_layer(kv_cache, layer)
+    if (key is None) != (value is None):
+        raise ValueError("key and value are given together")
+    if key is None:
+        _require_cuda(slot_mapping, "slot_mapping")
+        shape = (slot_mapping.numel(), kv_cache.size(2), 128)
+        key = torch.empty(shape, dtype=kv_cache.dtype, device=kv_cache.device)
+        value = torch.empty_like(key)
+    elif key.dim() != 3 or key.size(1) != kv_cache.size(2):
+        raise ValueError("key and value must be [T, Hkv, 128] with the cache's Hkv")
+    _int4_rows(key, value, kv_cache, slot_mapping)
+    slot_mapping = slot_mapping.contiguous()
+    dev = kv_cache.device
+    with torch.cuda.device(dev):
+        st = lib.aeg_gather_cache_int4(key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0), base,
+                                       kv_cache.stride(0), kv_cache.size(0), slot_mapping.data_ptr(), key.size(0),
+                                       key.size(1), key.size(2), _DTYPES[kv_cache.dtype], _stream(dev))
+    check(st, "gather_cache_int4")
+    return key, value
+
+
+# --------------------------------------------------------------------------------------------
+# Rotary positions with several axes
+
+
+@functools.lru_cache(maxsize=64)
+def _axis_of(sections: tuple[int, ...], interleaved: bool) -> bytes:
+    """The axis of each frequency, one byte each."""
+    if not 1 <= len(sections) <= 4 or any(n < 0 for n in sections) or sum(sections) < 1:
+        raise ValueError(f"sections must be 1 to 4 non-negative counts of frequencies, got {sections}")
+    if not interleaved:
+        return bytes(a for a, n in enumerate(sections) for _ in range(n))
+    left, order = list(sections), []
+    while any(left):
+        for a, n in enumerate(left):
+            if n:
+                left[a] -= 1
+                order.append(a)
+    return bytes(order)
+
+
+def rotary_multi_axis(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                      sections: Sequence[int], *, interleaved: bool = False, scaling: float = 1.0,
+                      query_out: torch.Tensor | None = None,
+                      key_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rotates ``query`` ``[T, Hq, D]`` and ``key`` ``[T, Hkv, D]`` (fp16 or bf16, any token stride) by
+    positions with up to four axes (time, height, width of image and video tokens).
+
+    ``positions`` int64 ``[axes, T]`` (``[T]`` for one axis, as ``prepare_step_inputs`` gives them),
+    ``inv_freq`` float32 ``[half]``; ``sections[a]`` frequencies belong to axis a: one section after
+    another, or with ``interleaved=True`` dealt to the axes in turn until an axis has its number. Pairs
+    are dims (i, i + half); dims from ``2 * half`` on are copied. ``scaling`` multiplies the rotated
+    dims. Returns new tensors unless ``query_out``/``key_out`` are given; those may be the inputs.
+    """
+    for name, t in (("query", query), ("key", key)):
+        _require_cuda(t, name)
+        if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.size(2):
+            raise ValueError(f"{name} must be [T, heads, D] with contiguous heads")
+    if query.dtype not in _DTYPES or key.dtype != query.dtype:
+        raise ValueError("query and key must share an fp16 or bf16 dtype")
+    T, Hq, D = query.shape
+    if key.size(0) != T or key.size(2) != D:
+        raise ValueError("query and key must have the same tokens and head_dim")
+    axis_of = _axis_of(tuple(sections), bool(interleaved))
+    half = len(axis_of)
+    _require_cuda(positions, "positions")
+    _require_cuda(inv_freq, "inv_freq")
+    if positions.dim() == 1:
+        positions = positions.unsqueeze(0)
+    if positions.dtype != torch.int64 or tuple(positions.shape) != (len(sections), T):
+        raise ValueError(f"positions must be int64 [{len(sections)}, {T}]")
+    if positions.stride(1) != 1 or positions.stride(0) < T:
+        positions = positions.contiguous()
+    if inv_freq.dtype != torch.float32 or inv_freq.shape != (half,):
+        raise ValueError(f"inv_freq must be float32 [{half}], one per frequency of the sections")
+    inv_freq = inv_freq.contiguous()
+    if query_out is None:
+        query_out = torch.empty((T, Hq, D), dtype=query.dtype, device=query.device)
+    if key_out is None:
+        key_out = torch.empty(key.shape, dtype=key.dtype, device=key.device)
+    for name, out, src in (("query_out", query_out, query), ("key_out", key_out, key)):
+        if out.shape != src.shape or out.dtype != src.dtype or out.stride(2) != 1 or out.stride(1) != D:
+            raise ValueError(f"{name} must match its input's shape and dtype, with contiguous heads")
+        if out.data_ptr() == src.data_ptr() and out.stride(0) != src.stride(0):
+            raise ValueError(f"{name} shares its input's memory with another stride")
+    dev = query.device
+    _same_device(dev, key=key, positions=positions, inv_freq=inv_freq, query_out=query_out, key_out=key_out)
+    with torch.cuda.device(dev):
+        st = lib.aeg_rotary_multi_axis(query_out.data_ptr(), query_out.stride(0), key_out.data_ptr(), key_out.stride(0),
+                                       query.data_ptr(), query.stride(0), key.data_ptr(), key.stride(0),
+                                       positions.data_ptr(), positions.stride(0), len(sections), inv_freq.data_ptr(),
+                                       axis_of, half, float(scaling), T, Hq, key.size(1), D, _DTYPES[query.dtype],
+                                       _stream(dev))
+    check(st, "rotary_multi_axis")
+    return query_out, key_out
+
+
+# --------------------------------------------------------------------------------------------
+# Shared blocks: forking, freeing and compacting over reference counts
+
+
+def _check_shared(ref_counts: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor) -> torch.device:
+    for t, name in ((ref_counts, "ref_counts"), (block_tables, "block_tables"), (seq_lens, "seq_lens")):
+        _require_cuda(t, name)
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor")
+    if ref_counts.dim() != 1 or block_tables.dim() != 2 or seq_lens.dim() != 1:
+        raise ValueError("ref_counts must be [num_blocks], block_tables [rows, W] and seq_lens [rows]")
+    if seq_lens.numel() != block_tables.size(0):
+        raise ValueError("seq_lens must have one entry per table row")
+    if block_tables.size(1) == 0:
+        raise ValueError("block_tables has no columns")
+    dev = ref_counts.device
+    _same_device(dev, block_tables=block_tables, seq_lens=seq_lens)
+    return dev
+
+
+def _check_pool(kv_cache: torch.Tensor, ref_counts: torch.Tensor) -> None:
+    _require_cuda(kv_cache, "kv_cache")
+    if not kv_cache.is_contiguous() or kv_cache.dim() < 1:
+        raise ValueError("kv_cache must be contiguous")
+    if kv_cache.size(0) != ref_counts.numel():
+        raise ValueError(f"kv_cache has {kv_cache.size(0)} blocks but ref_counts {ref_counts.numel()} entries")
+    _same_device(ref_counts.device, kv_cache=kv_cache)
+
+
+def fork_blocks(kv_cache: torch.Tensor, ref_counts: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                src_rows, dst_rows) -> torch.Tensor:
+    """Turns the empty table row ``dst_rows[i]`` into a fork of row ``src_rows[i]`` (a parallel sample or
+    a beam): full blocks are shared (``ref_counts`` goes up), a partly filled last block is copied into
+    the lowest free block.
+
+    ``kv_cache`` is any block pool (16-bit or 4-bit, one entry of dim 0 per block), ``ref_counts``
+    int32 ``[num_blocks]`` (0 = free), ``block_tables`` int32 ``[rows, W]``, ``seq_lens`` int32 ``[rows]``
+    (0 = empty row); ``kv_cache``, ``ref_counts``, ``block_tables`` and ``seq_lens`` are updated in place
+    on the current stream, without reading anything back. Returns int32 ``[n]``: the block each fork
+    took, or -1. Refused entries leave their row empty and raise a device error
+    (``read_device_errors``): a row out of range, a target row that is not empty or named before, a
+    pool with no free block left.
+    """
+    dev = _check_shared(ref_counts, block_tables, seq_lens)
+    _check_pool(kv_cache, ref_counts)
+    src = _device_ids(src_rows, dev, "src_rows")
+    dst = _device_ids(dst_rows, dev, "dst_rows")
+    n = src.numel()
+    if dst.numel() != n:
+        raise ValueError(f"{n} source rows but {dst.numel()} target rows")
+    new_blocks = torch.empty(n, dtype=torch.int32, device=dev)
+    if n == 0:
+        return new_blocks
+    ws = torch.empty(lib.aeg_fork_blocks_workspace_size(n), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        st = lib.aeg_fork_blocks(kv_cache.data_ptr(), block_bytes(kv_cache), ref_counts.numel(), ref_counts.data_ptr(),
+                                 block_tables.data_ptr(), block_tables.size(1), block_tables.size(0),
+                                 seq_lens.data_ptr(), src.data_ptr(), dst.data_ptr(), n, new_blocks.data_ptr(),
+                                 ws.data_ptr(), ws.numel(), _stream(dev))
+    check(st, "fork_blocks")
+    return new_blocks
+
+
+def free_blocks(ref_counts: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, rows) -> None:
+    """Empties the table rows ``rows``: every block of a row gives back one reference (a block at 0 is
+    free), and the row's length becomes 0. A row named twice is freed once."""
+    dev = _check_shared(ref_counts, block_tables, seq_lens)
+    ids = _device_ids(rows, dev, "rows")
+    if ids.numel() == 0:
+        return
+    with torch.cuda.device(dev):
+        st = lib.aeg_free_blocks(ref_counts.numel(), ref_counts.data_ptr(), block_tables.data_ptr(),
+                                 block_tables.size(1), block_tables.size(0), seq_lens.data_ptr(), ids.data_ptr(),
+                                 ids.numel(), _stream(dev))
+    check(st, "free_blocks")
+
+
+class CompactedBlocks(NamedTuple):
+    """What ``compact_blocks`` returns (device tensors)."""
+    block_tables: torch.Tensor  # int32 [rows, W], the tables with the new ids
+    ref_counts: torch.Tensor    # int32 [num_blocks], of the new ids
+    remap: torch.Tensor         # int32 [num_blocks], old id -> new id, -1 for a free block
+    num_live: torch.Tensor      # int32 [1]: ids 0 .. num_live - 1 are live, all others free
+
+
+def compact_blocks(kv_cache: torch.Tensor, ref_counts: torch.Tensor, block_tables: torch.Tensor,
+                   seq_lens: torch.Tensor) -> CompactedBlocks:
+    """Moves a fragmented pool's live blocks to its lowest ids, so that its tail can be given to another
+    model, on the current stream and without reading anything back.
+
+    The live blocks' contents are copied within ``kv_cache``: the k-th live id that is not below the
+    number of live blocks goes to the k-th free id below it. ``ref_counts``, ``block_tables`` and
+    ``seq_lens`` are only read: adopt the returned tables and counts. The old places keep their
+    contents, so a step in flight on the old tables stays right until their ids are given out.
+    """
+    dev = _check_shared(ref_counts, block_tables, seq_lens)
+    _check_pool(kv_cache, ref_counts)
+    N = ref_counts.numel()
+    out = CompactedBlocks(torch.empty_like(block_tables), torch.empty_like(ref_counts), torch.empty_like(ref_counts),
+                          torch.empty(1, dtype=torch.int32, device=dev))
+    ws = torch.empty(lib.aeg_compact_blocks_workspace_size(N), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        st = lib.aeg_compact_blocks(kv_cache.data_ptr(), block_bytes(kv_cache), N, ref_counts.data_ptr(),
+                                    block_tables.data_ptr(), block_tables.size(1), block_tables.size(0),
+                                    seq_lens.data_ptr(), out.ref_counts.data_ptr(), out.block_tables.data_ptr(),
+                                    out.remap.data_ptr(), out.num_live.data_ptr(), ws.data_ptr(), ws.numel(),
+                                    _stream(dev))
+    check(st, "compact_blocks")
+    return out
 
 
 # --------------------------------------------------------------------------------------------

@@ -71,6 +71,8 @@ typedef enum {
 #define AEG_DEVERR_SEQ_LEN_RANGE 0x4u  /* seq_len < 0 or > 16 * block-table width, clamped  */
 #define AEG_DEVERR_WAIT_TIMEOUT 0x8u   /* a bounded pipeline wait gave up (output invalid)   */
 #define AEG_DEVERR_PLAN_MISMATCH 0x10u /* the workspace plan does not fit this call; skipped  */
+#define AEG_DEVERR_POOL_ENTRY 0x20u    /* a fork/free entry was refused (aeg_fork_blocks)     */
+#define AEG_DEVERR_POOL_EMPTY 0x40u    /* no free block was left for a fork                   */
 
 /* Library version (major*10000 + minor*100 + patch). */
 AEG_API int aeg_version(void);
@@ -353,6 +355,104 @@ AEG_API int aeg_paged_attn_decode_noalloc(void* out, int64_t out_stride, const v
                                           const int32_t* block_tables, int table_stride,
                                           const int32_t* seq_lens, int B, int Hq, int Hkv, int D,
                                           float scale, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * A KV cache held in 4 bits (no counterpart in the reference, whose cache is fp16/bf16).
+ *
+ * kv_cache[num_blocks][L][Hkv][1152] elements of the model's 16-bit type (`dtype`): one tile of
+ * 2304 contiguous bytes holds 16 tokens of one (block, layer, KV head), D = 128: 4-bit key codes,
+ * 4-bit value codes, then a (scale, minimum) pair in `dtype` for each token and 64-dim group of
+ * the keys and of the values. An element stands for code * scale + minimum, where minimum is the
+ * group's least element, scale = (max - min) / 15 rounded once to `dtype` and code =
+ * (x - minimum) / scale rounded to the nearest whole number, ties to even, in 0 .. 15 (decided
+ * exactly, as if in infinite precision). A group whose max - min is not finite in fp32 (a NaN, an
+ * infinity, a spread beyond fp32) reads back as NaN. 144 bytes hold a token's keys and values of
+ * one head instead of 512. Whole blocks are contiguous, so aeg_copy_blocks, aeg_swap,
+ * aeg_migrate_blocks and the calls below on shared blocks move them like any other.
+ * `kv_cache` points at the layer's first tile; `block_stride` is the elements between blocks
+ * (L * Hkv * 1152). */
+
+/* aeg_reshape_and_cache for a 4-bit cache: for t < T with slot s = slot_mapping[t] >= 0, key[t]
+ * and value[t] ([Hkv, D], token strides in elements) are rounded into row s % 16 of block s / 16's
+ * tiles. Slots < 0 are skipped, slots >= num_blocks * 16 too, raising AEG_DEVERR_SLOT_RANGE. No
+ * other row changes. A slot must not occur twice in a call. */
+AEG_API int aeg_reshape_and_cache_int4(const void* key, const void* value, int64_t key_stride,
+                                       int64_t value_stride, void* kv_cache, int64_t block_stride,
+                                       int64_t num_blocks, const int64_t* slot_mapping, int64_t T,
+                                       int Hkv, int D, int dtype, void* stream);
+
+/* The read-back: key[t], value[t] = the values held at slot_mapping[t], rounded to `dtype`. Slots
+ * < 0 give zero rows, slots >= num_blocks * 16 too, raising AEG_DEVERR_SLOT_RANGE. */
+AEG_API int aeg_gather_cache_int4(void* key, void* value, int64_t key_stride, int64_t value_stride,
+                                  const void* kv_cache, int64_t block_stride, int64_t num_blocks,
+                                  const int64_t* slot_mapping, int64_t T, int Hkv, int D, int dtype,
+                                  void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Rotary positions with several axes (time, height, width of image and video tokens), applied to
+ * a step's queries and keys before the cache write and the attention. The reference reaches its
+ * model's rotary embedding through vLLM (aegaeon/aegaeon/worker.py:517-523).
+ *
+ * For i < half with a = axis_of[i] (HOST bytes, a < axes <= 4) and theta = positions[a][t] *
+ * inv_freq[i] (positions: DEVICE int64 [axes] rows `axis_stride` apart; inv_freq: DEVICE float):
+ *   out[t][h][i]        = scaling * (x[t][h][i] cos(theta) - x[t][h][i + half] sin(theta))
+ *   out[t][h][i + half] = scaling * (x[t][h][i + half] cos(theta) + x[t][h][i] sin(theta))
+ * for every head h of q [T, Hq, D] and k [T, Hkv, D] (token strides in elements, Hkv may be 0); dims
+ * from 2 * half on are copied. The angle is made and reduced in 64 bits. The outputs may be the
+ * inputs (same pointer and stride). half <= 128. */
+AEG_API int aeg_rotary_multi_axis(void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride,
+                                  const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                                  const int64_t* positions, int64_t axis_stride, int axes,
+                                  const float* inv_freq, const uint8_t* axis_of, int half,
+                                  float scaling, int64_t T, int Hq, int Hkv, int D, int dtype,
+                                  void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Shared blocks. The reference's BlockManager gives every request blocks of its own
+ * (aegaeon/aegaeon/block_manager.py); parallel samples and beams share their common prefix through
+ * these calls instead. All state is on the device and stays there:
+ *   ref_counts    int32 [num_blocks]      table rows that hold the block; 0 = free
+ *   block_tables  int32 [rows, table_stride], seq_lens int32 [rows]: row r holds the first
+ *                 ceil(seq_lens[r] / 16) entries of its table row; length 0 = an empty row
+ * Free blocks are taken lowest id first, in the order of the call's entries.
+ *
+ * aeg_fork_blocks: for i < n, the empty row d_dst_rows[i] becomes a copy of row d_src_rows[i] (its
+ * length, its blocks), sharing every full block; a partly filled last block, which both rows go on
+ * writing, is copied whole (block_bytes) into a free block. new_blocks[i] receives that block's id,
+ * or -1. An entry is refused (row untouched, new_blocks[i] = -1, AEG_DEVERR_POOL_ENTRY) when a row
+ * is outside the table, the source's length is outside it, the target row is not empty or an earlier
+ * entry names it; AEG_DEVERR_BLOCK_ID_RANGE instead when the block to copy is outside the pool, and
+ * AEG_DEVERR_POOL_EMPTY when no free block is left (later entries that need none still proceed).
+ * Sources are read as they were before the call. */
+AEG_API size_t aeg_fork_blocks_workspace_size(int64_t n);
+AEG_API int aeg_fork_blocks(void* pool, size_t block_bytes, int64_t num_blocks, int32_t* ref_counts,
+                            int32_t* block_tables, int table_stride, int rows, int32_t* seq_lens,
+                            const int64_t* d_src_rows, const int64_t* d_dst_rows, int64_t n,
+                            int32_t* new_blocks, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* aeg_free_blocks: the rows d_rows[0 .. n) become empty (length 0) and give back one reference to
+ * each of their blocks. A row named twice, or already empty, gives nothing back the second time. Rows
+ * outside the table are skipped; a block without references stays at 0; both raise
+ * AEG_DEVERR_POOL_ENTRY. */
+AEG_API int aeg_free_blocks(int64_t num_blocks, int32_t* ref_counts, const int32_t* block_tables,
+                            int table_stride, int rows, int32_t* seq_lens, const int64_t* d_rows,
+                            int64_t n, void* stream);
+
+/* aeg_compact_blocks: moves the live blocks (ref_counts > 0) to the ids below their number: the k-th
+ * live id from num_live on goes to the k-th free id below it, the others stay. Writes the new tables
+ * and counts, remap[old id] = new id (-1 for a free block) and *num_live; the inputs keep their
+ * values, and so do the moved blocks' old places, so that work in flight on the old tables stays
+ * right until those ids are given out again. block_tables_out may be block_tables. A table entry in
+ * use that is outside the pool or free is left as it is (AEG_DEVERR_BLOCK_ID_RANGE); a length outside
+ * the table is clamped (AEG_DEVERR_SEQ_LEN_RANGE). Pointers of outputs are DEVICE memory. */
+AEG_API size_t aeg_compact_blocks_workspace_size(int64_t num_blocks);
+AEG_API int aeg_compact_blocks(void* pool, size_t block_bytes, int64_t num_blocks,
+                               const int32_t* ref_counts, const int32_t* block_tables,
+                               int table_stride, int rows, const int32_t* seq_lens,
+                               int32_t* ref_counts_out, int32_t* block_tables_out, int32_t* remap,
+                               int32_t* num_live, void* workspace, size_t workspace_bytes,
+                               void* stream);
 
 #ifdef __cplusplus
 }
