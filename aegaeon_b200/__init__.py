@@ -15,6 +15,7 @@ __version__ = "0.1.0"
 _SUBMODULES = ("build", "layout", "ops", "step", "synth")
 _OPS_EXPORTS = ("DecodePlan", "compact_blocks", "copy_blocks", "decode_layer", "decode_layer_flash",
                 "flash_attn_decode", "fork_blocks", "free_blocks", "gather_cache_int4", "paged_attention_decode",
+                "paged_attention_decode_int4",
                 "read_device_errors", "reshape_and_cache", "reshape_and_cache_flash", "reshape_and_cache_int4",
                 "rotary_multi_axis", "swap", "swap_sm")
 

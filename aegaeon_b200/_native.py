@@ -78,6 +78,10 @@ SIGNATURES = {
                                           _i32, _i32, _i32, _c_void_p]),
     "aeg_gather_cache_int4": (_i32, [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i32,
                                      _i32, _i32, _c_void_p]),
+    "aeg_decode_plan_int4": (_i32, [_c_void_p, _sz, _c_void_p, _i32, _c_void_p, _i32, _i32, _i32, _i32, _c_void_p]),
+    "aeg_paged_attn_decode_int4": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64, _c_void_p, _i32,
+                                          _c_void_p, _i32, _i32, _i32, _i32, ctypes.c_float, _i32, _c_void_p, _sz, _i32,
+                                          _c_void_p]),
     "aeg_rotary_multi_axis": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,
                                      _i64, _i32, _c_void_p, _c_void_p, _i32, ctypes.c_float, _i64, _i32, _i32, _i32,
                                      _i32, _c_void_p]),

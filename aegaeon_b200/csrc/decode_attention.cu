@@ -47,6 +47,7 @@
 //   * Every wait is bounded (2 s); a timeout raises AEG_DEVERR_WAIT_TIMEOUT and the warp
 //     drains instead of hanging.
 #include "aeg_common.cuh"
+#include "int4_tile.cuh"
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -646,7 +647,7 @@ __device__ __forceinline__ void merge_small(const AttnParams& p, const int4& e, 
 //   * q > 1 (more than kMergeBatch pieces): the item is (head item / q, dimension chunk
 //     item % q); lane = (piece group g, float4 column c) with 32 / q columns per chunk, group g
 //     takes pieces g, g + q, ..., and the q groups are combined by xor shuffles.
-template <typename T>
+template <typename T, int kLoads = kMergeBatch>
 __device__ __forceinline__ void merge_item(const AttnParams& p, const int4& e, int item, int lane) {
   const int G = p.G;
   const int shape = e.z >> 16, q = shape & 0xff, hg = shape >> 8, ns = e.z & 0xffff;
@@ -691,24 +692,24 @@ __device__ __forceinline__ void merge_item(const AttnParams& p, const int4& e, i
   const int col = (chunk << lc) + c;  // float4 column of the 128-dim row
   float M = -INFINITY, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = g; s0 < ns; s0 += q * kMergeBatch) {
-    float2 ml[kMergeBatch];
-    float4 v[kMergeBatch];
-    const int cnt = min(kMergeBatch, (ns - s0 + q - 1) >> lq);
+  for (int s0 = g; s0 < ns; s0 += q * kLoads) {
+    float2 ml[kLoads];
+    float4 v[kLoads];
+    const int cnt = min(kLoads, (ns - s0 + q - 1) >> lq);
 #pragma unroll
-    for (int i = 0; i < kMergeBatch; ++i) {
+    for (int i = 0; i < kLoads; ++i) {
       if (i >= cnt) break;
       const int64_t row = static_cast<int64_t>(e.y + s0 + (i << lq)) * G + n;
       ml[i] = ld_cg_f2(&p.ws.part_ml[row]);
       v[i] = ld_cg_f4(po4 + row * (kHeadDim / 4) + col);
     }
 #pragma unroll
-    for (int i = 0; i < kMergeBatch; ++i) {
+    for (int i = 0; i < kLoads; ++i) {
       if (i >= cnt) break;
       after_loads(ml[i], v[i]);
     }
 #pragma unroll
-    for (int i = 0; i < kMergeBatch; ++i) {
+    for (int i = 0; i < kLoads; ++i) {
       if (i >= cnt) break;
       fold(M, L, acc, ml[i], v[i]);
     }
@@ -735,13 +736,13 @@ __device__ __forceinline__ void merge_item(const AttnParams& p, const int4& e, i
 }
 
 // A split-pair entry is used only if it fits this call's shape (see unit_items).
-__device__ __forceinline__ bool entry_ok(const int4& e, const AttnParams& p) {
+__device__ __forceinline__ bool entry_ok(const int4& e, const AttnParams& p, int total_warps) {
   const int shape = e.z >> 16, q = shape & 0xff, hg = shape >> 8, ns = e.z & 0xffff;
   const int w0 = e.w & 0xffff, n_w = e.w >> 16;
   const bool shape_ok = (q == 1 && hg == 4 && ns <= 4) || (q == 1 && hg == 1 && ns > 4 && ns <= kMergeBatch) ||
                         (hg == 1 && (q == 2 || q == 4 || q == 8 || q == 16 || q == 32));
   return e.x >= 0 && e.x < p.num_pairs && e.y >= 0 && e.y + ns <= p.max_slots && shape_ok &&
-         w0 + n_w <= static_cast<int>(gridDim.x) * kWarps && (ns == 0) == (n_w == 0);
+         w0 + n_w <= total_warps && (ns == 0) == (n_w == 0);
 }
 
 __device__ __forceinline__ void st_release_gpu(int* p, int v) {
@@ -1289,7 +1290,7 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         k = 0;
         me = entry < n_entries ? p.ws.split_pairs[entry] : none;
       }
-      if (!entry_ok(me, p) || k < 0) {
+      if (!entry_ok(me, p, total_warps) || k < 0) {
         if (lane == 0) atomicOr(&g_deverr_attn, AEG_DEVERR_PLAN_MISMATCH);
         break;
       }
@@ -1315,6 +1316,8 @@ decode_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
     atomicOr(&g_deverr_attn, AEG_DEVERR_PLAN_MISMATCH);
   }
 }
+
+#include "decode_attention_int4.cuh"
 
 // ---------------------------------------------------------------------------------------
 // Host side: tensor maps, launch configuration.
@@ -1438,6 +1441,57 @@ int launch_attn_t(const CUtensorMap& km, const CUtensorMap& vm, const AttnParams
 int worker_warps(int G) {
   const int per_sm = ctas_per_sm(AEG_DTYPE_FP16, G <= 8 ? 1 : 2);
   return num_sms() * (per_sm > 0 ? per_sm : 1) * kWarps;
+}
+
+// The same for the kernel over a 4-bit cache: one CTA per SM by its shared memory.
+template <typename T, int NT>
+int check_attn_int4(int max_warps) {
+  using SL = Int4Smem<NT>;
+  static std::mutex mu;
+  static int ctas[64] = {0};
+  int dev = 0;
+  AEG_CHECK_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return set_error(AEG_ERR_UNSUPPORTED, "decode_int4: device ordinal %d >= 64", dev);
+  std::lock_guard<std::mutex> lock(mu);
+  if (ctas[dev] == 0) {
+    auto kern = decode_attn_int4_kernel<T, NT>;
+    int n = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SL::kDynamic)) !=
+            cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, SL::kThreads, SL::kDynamic) != cudaSuccess || n < 1) {
+      (void)cudaGetLastError();
+      return set_error(AEG_ERR_CUDA, "decode_int4: the kernel cannot be configured on this device");
+    }
+    ctas[dev] = n;
+  }
+  if (num_sms() * SL::kWarps > max_warps)
+    return set_error(AEG_ERR_UNSUPPORTED, "decode_int4: %d worker warps exceed the workspace's %d", num_sms() * SL::kWarps,
+                     max_warps);
+  return AEG_OK;
+}
+
+int worker_warps_int4(int G) { return num_sms() * (G <= 8 ? Int4Smem<1>::kWarps : Int4Smem<2>::kWarps); }
+
+template <typename T, int NT>
+int launch_attn_int4(const AttnParams& prm, cudaStream_t stream, cudaEvent_t started) {
+  cudaLaunchAttribute attr[2] = {pdl_attr(), cudaLaunchAttribute{}};
+  unsigned n_attr = 1;
+  if (started != nullptr) {
+    attr[1].id = cudaLaunchAttributeProgrammaticEvent;
+    attr[1].val.programmaticEvent.event = started;
+    attr[1].val.programmaticEvent.flags = 0;
+    attr[1].val.programmaticEvent.triggerAtBlockStart = 1;
+    n_attr = 2;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(num_sms()));
+  cfg.blockDim = dim3(Int4Smem<NT>::kThreads);
+  cfg.dynamicSmemBytes = Int4Smem<NT>::kDynamic;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = n_attr;
+  AEG_CHECK_CUDA(cudaLaunchKernelEx(&cfg, decode_attn_int4_kernel<T, NT>, prm));
+  return AEG_OK;
 }
 
 int validate_shape(int B, int Hq, int Hkv, int D, int table_stride) {
@@ -1649,6 +1703,84 @@ int decode_common(void* out, int64_t out_stride, const void* q, int64_t q_stride
   return decode_launch(dl, s, order);
 }
 
+// Decode attention over a 4-bit cache.
+int decode_int4(void* out, int64_t out_stride, const void* q, int64_t q_stride, const void* kv_cache, int64_t block_stride,
+                int64_t num_blocks, const int32_t* block_tables, int table_stride, const int32_t* seq_lens, int B, int Hq,
+                int Hkv, int D, float scale, int dtype, void* workspace, size_t workspace_bytes, int flags, void* stream) {
+  int st = validate_shape(B, Hq, Hkv, D, table_stride);
+  if (st != AEG_OK || B == 0) return st;
+  const WsLayout L = ws_layout(B, Hq, Hkv, D);
+  AEG_CHECK_ARG(dtype == AEG_DTYPE_FP16 || dtype == AEG_DTYPE_BF16, "decode_int4: dtype %d is not fp16/bf16", dtype);
+  AEG_CHECK_ARG(out && q && kv_cache && block_tables && seq_lens, "decode_int4: null pointer");
+  AEG_CHECK_ARG(workspace != nullptr && aligned(workspace, 256), "decode_int4: workspace must be 256-byte aligned");
+  AEG_CHECK_ARG(workspace_bytes >= L.total, "decode_int4: workspace of %zu bytes, need %zu", workspace_bytes, L.total);
+  AEG_CHECK_ARG(num_blocks > 0 && num_blocks <= 0x7fffffffLL, "decode_int4: num_blocks %lld out of range",
+                (long long)num_blocks);
+  AEG_CHECK_ARG(aligned(kv_cache, 16), "decode_int4: the cache must be 16-byte aligned");
+  AEG_CHECK_ARG(block_stride % 8 == 0 && block_stride >= int64_t(Hkv) * kInt4TileElems,
+                "decode_int4: block stride %lld must be a multiple of 8 elements and >= Hkv*1152", (long long)block_stride);
+  AEG_CHECK_ARG(q_stride >= int64_t(Hq) * D && out_stride >= int64_t(Hq) * D, "decode_int4: q/out token stride < Hq*D");
+  AEG_CHECK_ARG(aligned(q, 4) && q_stride % 2 == 0, "decode_int4: q must be 4-byte aligned with an even token stride");
+  AEG_CHECK_ARG(aligned(out, 2), "decode_int4: out must be 2-byte aligned");
+  AEG_CHECK_ARG(aligned(block_tables, 4) && aligned(seq_lens, 4), "decode_int4: int32 arrays must be aligned");
+  AEG_CHECK_ARG((flags & ~AEG_DECODE_PREFETCH) == 0, "decode_int4: flags 0x%x, only AEG_DECODE_PREFETCH is known", flags);
+  const bool one = Hq / Hkv <= 8, bf = dtype == AEG_DTYPE_BF16;
+  st = bf ? (one ? check_attn_int4<__nv_bfloat16, 1>(L.max_warps) : check_attn_int4<__nv_bfloat16, 2>(L.max_warps))
+          : (one ? check_attn_int4<__half, 1>(L.max_warps) : check_attn_int4<__half, 2>(L.max_warps));
+  if (st != AEG_OK) return st;
+  AttnParams prm{};
+  prm.out = out;
+  prm.out_stride = out_stride;
+  prm.q = q;
+  prm.q_stride = q_stride;
+  prm.tables = block_tables;
+  prm.table_stride = table_stride;
+  prm.seq_lens = seq_lens;
+  prm.G = Hq / Hkv;
+  prm.Hkv = Hkv;
+  prm.num_pairs = B * Hkv;
+  prm.max_warps = L.max_warps;
+  prm.max_units = L.max_units;
+  prm.max_slots = L.max_slots;
+  prm.num_blocks = num_blocks;
+  prm.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);  // log2(e)
+  prm.q_bulk = (aligned(q, 16) && q_stride % 8 == 0) ? 1 : 0;
+  prm.k_cache = const_cast<void*>(kv_cache);
+  prm.block_stride = block_stride;
+  prm.ws = ws_ptrs(workspace, L);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  LaunchOrder order;
+  bool waited = false;
+  st = order.enter(s, &waited);
+  if (st != AEG_OK) return st;
+  prm.plan_ready = take_plan_fresh(workspace) ? 0 : 1;
+  prm.prefetch_kv = (flags & AEG_DECODE_PREFETCH) && !waited ? 1 : 0;
+  cudaEvent_t ev = order.event();
+  st = bf ? (one ? launch_attn_int4<__nv_bfloat16, 1>(prm, s, ev) : launch_attn_int4<__nv_bfloat16, 2>(prm, s, ev))
+          : (one ? launch_attn_int4<__half, 1>(prm, s, ev) : launch_attn_int4<__half, 2>(prm, s, ev));
+  if (st == AEG_OK) order.launched();
+  return st;
+}
+
+int plan_common(const char* what, void* workspace, size_t workspace_bytes, const int32_t* block_tables, int table_stride,
+                const int32_t* seq_lens, int B, int Hq, int Hkv, int D, bool int4, void* stream) {
+  int st = validate_shape(B, Hq, Hkv, D, table_stride);
+  if (st != AEG_OK) return st;
+  AEG_CHECK_ARG(workspace != nullptr && aligned(workspace, 256), "%s: workspace must be 256-byte aligned", what);
+  const WsLayout L = ws_layout(B, Hq, Hkv, D);
+  AEG_CHECK_ARG(workspace_bytes >= L.total, "%s: workspace of %zu bytes, need %zu", what, workspace_bytes, L.total);
+  AEG_CHECK_ARG(B == 0 || (seq_lens != nullptr && block_tables != nullptr), "%s: seq_lens/block_tables is NULL", what);
+  AEG_CHECK_ARG(aligned(seq_lens, 4) && aligned(block_tables, 4), "%s: int32 arrays must be aligned", what);
+  const int W = int4 ? worker_warps_int4(Hq / Hkv) : worker_warps(Hq / Hkv);
+  if (W > L.max_warps)
+    return set_error(AEG_ERR_UNSUPPORTED, "%s: %d worker warps exceed the workspace's %d", what, W, L.max_warps);
+  decode_plan_kernel<<<1, kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(seq_lens, block_tables, B, Hkv, Hq / Hkv,
+                                                                                 table_stride, W, ws_ptrs(workspace, L));
+  AEG_CHECK_LAUNCH(what);
+  mark_plan_fresh(workspace);
+  return AEG_OK;
+}
+
 // ---------------------------------------------------------------------------------------
 // Allocation-free decode attention (aeg_paged_attn_decode_noalloc).
 //
@@ -1736,22 +1868,22 @@ size_t aeg_decode_workspace_size(int B, int Hq, int Hkv, int D) {
 
 int aeg_decode_plan(void* workspace, size_t workspace_bytes, const int32_t* block_tables, int table_stride,
                     const int32_t* seq_lens, int B, int Hq, int Hkv, int D, void* stream) {
-  int st = aeg::validate_shape(B, Hq, Hkv, D, table_stride);
-  if (st != AEG_OK) return st;
-  AEG_CHECK_ARG(workspace != nullptr && aeg::aligned(workspace, 256), "decode_plan: workspace must be 256-byte aligned");
-  const aeg::WsLayout L = aeg::ws_layout(B, Hq, Hkv, D);
-  AEG_CHECK_ARG(workspace_bytes >= L.total, "decode_plan: workspace of %zu bytes, need %zu", workspace_bytes, L.total);
-  AEG_CHECK_ARG(B == 0 || (seq_lens != nullptr && block_tables != nullptr), "decode_plan: seq_lens/block_tables is NULL");
-  AEG_CHECK_ARG(aeg::aligned(seq_lens, 4) && aeg::aligned(block_tables, 4), "decode_plan: int32 arrays must be aligned");
-  const int W = aeg::worker_warps(Hq / Hkv);
-  if (W > L.max_warps)
-    return aeg::set_error(AEG_ERR_UNSUPPORTED, "decode_plan: %d worker warps exceed the workspace's %d", W, L.max_warps);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  aeg::WsPtrs w = aeg::ws_ptrs(workspace, L);
-  aeg::decode_plan_kernel<<<1, aeg::kPlanThreads, 0, s>>>(seq_lens, block_tables, B, Hkv, Hq / Hkv, table_stride, W, w);
-  AEG_CHECK_LAUNCH("decode_plan");
-  aeg::mark_plan_fresh(workspace);
-  return AEG_OK;
+  return aeg::plan_common("decode_plan", workspace, workspace_bytes, block_tables, table_stride, seq_lens, B, Hq, Hkv, D,
+                          false, stream);
+}
+
+int aeg_decode_plan_int4(void* workspace, size_t workspace_bytes, const int32_t* block_tables, int table_stride,
+                         const int32_t* seq_lens, int B, int Hq, int Hkv, int D, void* stream) {
+  return aeg::plan_common("decode_plan_int4", workspace, workspace_bytes, block_tables, table_stride, seq_lens, B, Hq, Hkv,
+                          D, true, stream);
+}
+
+int aeg_paged_attn_decode_int4(void* out, int64_t out_stride, const void* q, int64_t q_stride, const void* kv_cache,
+                               int64_t block_stride, int64_t num_blocks, const int32_t* block_tables, int table_stride,
+                               const int32_t* seq_lens, int B, int Hq, int Hkv, int D, float scale, int dtype,
+                               void* workspace, size_t workspace_bytes, int flags, void* stream) {
+  return aeg::decode_int4(out, out_stride, q, q_stride, kv_cache, block_stride, num_blocks, block_tables, table_stride,
+                          seq_lens, B, Hq, Hkv, D, scale, dtype, workspace, workspace_bytes, flags, stream);
 }
 
 int aeg_paged_attn_decode(void* out, int64_t out_stride, const void* q, int64_t q_stride, const void* k_cache,

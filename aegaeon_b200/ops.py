@@ -814,11 +814,15 @@ class DecodePlan:
 
     The plan depends only on ``seq_lens`` (like the per-step attention metadata of
     ``aegaeon/aegaeon/worker.py:694-711``). Its workspace is device memory owned by this object;
-    one plan must not be used by two streams at the same time.
+    one plan must not be used by two streams at the same time. ``cache="int4"`` plans for
+    ``paged_attention_decode_int4``, ``"auto"`` for the calls on 16-bit caches.
     """
 
     def __init__(self, batch: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
-                 device: torch.device | str = "cuda"):
+                 device: torch.device | str = "cuda", cache: str = "auto"):
+        if cache not in ("auto", "int4"):
+            raise ValueError(f"cache must be 'auto' or 'int4', not {cache!r}")
+        self.cache = cache
         self.batch, self.num_q_heads, self.num_kv_heads, self.head_dim = batch, num_q_heads, num_kv_heads, head_dim
         self.device = torch.device(device)
         if self.device.type != "cuda":
@@ -848,10 +852,11 @@ class DecodePlan:
         seq_lens = seq_lens.contiguous()
         if block_tables.stride(1) != 1:
             block_tables = block_tables.contiguous()
+        plan = lib.aeg_decode_plan_int4 if self.cache == "int4" else lib.aeg_decode_plan
         with torch.cuda.device(self.device):
-            st = lib.aeg_decode_plan(self.workspace.data_ptr(), self.workspace.numel(), block_tables.data_ptr(),
-                                     block_tables.stride(0), seq_lens.data_ptr(), self.batch, self.num_q_heads,
-                                     self.num_kv_heads, self.head_dim, _stream(self.device))
+            st = plan(self.workspace.data_ptr(), self.workspace.numel(), block_tables.data_ptr(), block_tables.stride(0),
+                      seq_lens.data_ptr(), self.batch, self.num_q_heads, self.num_kv_heads, self.head_dim,
+                      _stream(self.device))
         check(st, "decode_plan")
         self.table_width = block_tables.size(1)
         self.seq_lens = seq_lens
@@ -868,8 +873,9 @@ class DecodePlan:
         keys = ("items", "workers", "units", "split_pair_entries", "partial_slots", "merge_items")
         return dict(zip(keys, words))
 
-    def matches(self, B: int, Hq: int, Hkv: int, D: int, block_table: torch.Tensor, seq_lens: torch.Tensor) -> bool:
-        return ((self.batch, self.num_q_heads, self.num_kv_heads, self.head_dim) == (B, Hq, Hkv, D)
+    def matches(self, B: int, Hq: int, Hkv: int, D: int, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                cache: str = "auto") -> bool:
+        return ((self.batch, self.num_q_heads, self.num_kv_heads, self.head_dim, self.cache) == (B, Hq, Hkv, D, cache)
                 and self.block_tables is not None and self.block_tables.data_ptr() == block_table.data_ptr()
                 and self.seq_lens.data_ptr() == seq_lens.data_ptr() and self.table_width == block_table.size(1))
 
@@ -1022,3 +1028,54 @@ def paged_attention_decode(out: torch.Tensor, query: torch.Tensor, kv_cache: tor
     kc, vc = _layer_views(kv_cache, layer)
     flash_attn_decode(query, kc, vc, block_tables, seq_lens, scale, out=out, plan=plan, prefetch=prefetch,
                       after_decode_write=after_decode_write)
+
+
+def paged_attention_decode_int4(out: torch.Tensor, query: torch.Tensor, kv_cache: torch.Tensor, layer: int,
+                                block_tables: torch.Tensor, seq_lens: torch.Tensor, scale: float,
+                                plan: DecodePlan | None = None, prefetch: bool = False) -> None:
+    """Decode attention of ``layer`` over a 4-bit cache ``(N, L, Hkv, 1152)`` of the query's dtype
+    (``layout.int4_block_shape``, written by ``reshape_and_cache_int4``), into ``out``.
+
+    Arguments as for ``paged_attention_decode``; ``plan`` is a ``DecodePlan(..., cache="int4")`` built
+    for these tables and lengths. ``prefetch=True`` promises that the kernel launched just before on
+    this stream writes neither this layer's blocks nor the block tables (so not right after the
+    layer's ``reshape_and_cache_int4``).
+    """
+    _require_cuda(query, "query")
+    if query.dim() != 3 or query.stride(2) != 1 or query.stride(1) != query.size(2):
+        raise ValueError("query must be [B, Hq, D] with contiguous heads")
+    B, Hq, D = query.shape
+    base = _int4_layer(kv_cache, layer)
+    Hkv = kv_cache.size(2)
+    if query.dtype != kv_cache.dtype:
+        raise ValueError(f"query dtype {query.dtype} differs from cache dtype {kv_cache.dtype}")
+    _require_cuda(block_tables, "block_tables")
+    _require_cuda(seq_lens, "seq_lens")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.size(0) != B:
+        raise ValueError("block_tables must be int32 [B, W]")
+    if block_tables.stride(1) != 1:
+        block_tables = block_tables.contiguous()
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != (B,):
+        raise ValueError("seq_lens must be int32 [B]")
+    seq_lens = seq_lens.contiguous()
+    _require_cuda(out, "out")
+    if out.shape != query.shape or out.dtype != query.dtype or out.stride(2) != 1 or out.stride(1) != D:
+        raise ValueError("out must match query's shape/dtype with contiguous heads")
+    if B == 0:
+        return
+    if block_tables.size(1) == 0:
+        raise ValueError("block_tables has no columns")
+    if plan is None:
+        plan = DecodePlan(B, Hq, Hkv, D, query.device, cache="int4").plan(seq_lens, block_tables)
+    elif not plan.matches(B, Hq, Hkv, D, block_tables, seq_lens, "int4"):
+        raise ValueError("plan was built for a different batch / head layout / block tables / sequence lengths / cache")
+    dev = query.device
+    _same_device(dev, kv_cache=kv_cache, block_tables=block_tables, seq_lens=seq_lens, out=out,
+                 plan_workspace=plan.workspace)
+    with torch.cuda.device(dev):
+        st = lib.aeg_paged_attn_decode_int4(out.data_ptr(), out.stride(0), query.data_ptr(), query.stride(0), base,
+                                            kv_cache.stride(0), kv_cache.size(0), block_tables.data_ptr(),
+                                            block_tables.stride(0), seq_lens.data_ptr(), B, Hq, Hkv, D, float(scale),
+                                            _DTYPES[query.dtype], plan.workspace.data_ptr(), plan.workspace.numel(),
+                                            AEG_DECODE_PREFETCH if prefetch else 0, _stream(dev))
+    check(st, "paged_attention_decode_int4")

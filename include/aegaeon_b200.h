@@ -388,6 +388,22 @@ AEG_API int aeg_gather_cache_int4(void* key, void* value, int64_t key_stride, in
                                   const int64_t* slot_mapping, int64_t T, int Hkv, int D, int dtype,
                                   void* stream);
 
+/* aeg_paged_attn_decode over a 4-bit cache: the same result for the values the cache holds (their
+ * products and sums in fp32, the output rounded to `dtype` once; a row that reads back as NaN gives
+ * NaN). The workspace is planned by aeg_decode_plan_int4 (same size and arguments as aeg_decode_plan;
+ * a plan of the other kind raises AEG_DEVERR_PLAN_MISMATCH). A block id outside the pool raises
+ * AEG_DEVERR_BLOCK_ID_RANGE and its tokens are left out. flags: 0 or AEG_DECODE_PREFETCH. D = 128,
+ * Hq / Hkv <= 16, `kv_cache` 16-byte aligned. */
+AEG_API int aeg_decode_plan_int4(void* workspace, size_t workspace_bytes, const int32_t* block_tables,
+                                 int table_stride, const int32_t* seq_lens, int B, int Hq, int Hkv,
+                                 int D, void* stream);
+AEG_API int aeg_paged_attn_decode_int4(void* out, int64_t out_stride, const void* q, int64_t q_stride,
+                                       const void* kv_cache, int64_t block_stride, int64_t num_blocks,
+                                       const int32_t* block_tables, int table_stride,
+                                       const int32_t* seq_lens, int B, int Hq, int Hkv, int D,
+                                       float scale, int dtype, void* workspace, size_t workspace_bytes,
+                                       int flags, void* stream);
+
 /* ---------------------------------------------------------------------------------------
  * Rotary positions with several axes (time, height, width of image and video tokens), applied to
  * a step's queries and keys before the cache write and the attention. The reference reaches its
