@@ -3,9 +3,7 @@
 // the 16-bit kernel; what differs is how a worker warp fetches and computes a tile.
 //
 //   * A (block, head) tile of keys, values and pairs (int4_tile.cuh) is 2304 contiguous bytes: one
-//     untiled bulk copy a tile, kStages of them ahead of the compute in each warp's ring. Without a
-//     tensor map there is no zero fill, so a tile whose block id is outside the pool is not fetched
-//     (its barrier completes at once) and not computed.
+//     untiled bulk copy a tile, up to kStages of them ahead of the compute in each warp's ring.
 //   * No element is dequantised. With K = s c + m per (token, group) and c a whole number 0..15,
 //       q . K = sum over groups of  s (q . c) + m (sum of q)
 //       sum_t p_t V_t = sum_t (p_t s_t) c_t + sum_t p_t m_t
@@ -28,27 +26,30 @@
 //     share is therefore taken out of O, which leaves sums of the size of the result.
 //   * The running maximum moves only when a score exceeds it by kSlack (log2 units): sums are fp32, and
 //     most tiles need one vote instead of a reduction over the tokens and a rescaling of O.
-//   * Tiles are requested several at a time, one lane each, so that walking the units and the block
-//     table costs a fraction of an instruction stream a tile.
+//   * One warp of the CTA requests the tiles of all others, a lane for each, so that walking the units
+//     and the block table costs the computing warps neither instructions nor registers.
 //
 // What bounds it: at 4.5 bits an element the work per byte is 3.6 times that of the 16-bit kernel,
 // so issue slots count as much as bytes.
 
 template <int NT>
 struct Int4Smem {
-  // More worker warps than the 16-bit kernel's 8 hide the latency of a tile's longer chain, as far
-  // as the registers of one CTA per SM go.
-  static constexpr int kWarps = NT == 1 ? 12 : 8;
-  static constexpr int kThreads = kWarps * 32;
-  static constexpr int kStages = NT == 1 ? 7 : 10;
-  static constexpr int kBatch = kStages / 2;  // free stages at which a warp requests more
+  // Worker warps (the plan's workers) and one warp that requests their tiles, one lane a worker.
+  static constexpr int kWarps = NT == 1 ? 11 : 7;
+  static constexpr int kThreads = (kWarps + 1) * 32;
+  static constexpr int kStages = NT == 1 ? 8 : 11;
   static constexpr int kMergeLoads = NT == 1 ? 8 : kMergeBatch;  // pieces of a merge in flight per lane
   static constexpr int kQSlot = 8 * NT * kHeadDim * 2;
-  static constexpr int kPerWarp = kStages * kInt4TileBytes + kQSlot;
-  static constexpr int kOffBars = kWarps * kPerWarp;
-  static constexpr int kBarsPerWarp = kStages + 2;  // stages, query slot, one scratch word
-  static constexpr int kTotal = kOffBars + kWarps * kBarsPerWarp * 8;
-  static constexpr size_t kDynamic = size_t(kTotal) + 128;  // + alignment slack
+  static constexpr int kRing = kStages * kInt4TileBytes;
+  static constexpr int kPerWarp = kRing + kQSlot;
+  // Per worker: barriers (tile landed / free for each stage, queries landed / free), tokens of each
+  // stage's tile, and the record of the unit whose queries lie in the slot.
+  static constexpr int kBars = 2 * kStages + 2;
+  static constexpr int kTokens = 8 * kBars;
+  static constexpr int kRecord = (kTokens + 4 * kStages + 15) / 16 * 16;
+  static constexpr int kMeta = kRecord + 16;
+  static constexpr int kOffMeta = kWarps * kPerWarp;
+  static constexpr size_t kDynamic = size_t(kOffMeta) + kWarps * kMeta + 128;  // + alignment slack
   static_assert(kPerWarp % 128 == 0 && kDynamic <= 232448, "ring alignment and capacity");
 };
 
@@ -58,25 +59,25 @@ __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t b
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
   return r;
 }
-// Nibbles k and k + 4 (k = 0..3) of a key word as two elements of T, code + kKeyBias<T>.
-template <typename T>
-__device__ __forceinline__ uint32_t key_pair(uint32_t w, int k);
-template <>
-__device__ __forceinline__ uint32_t key_pair<__half>(uint32_t w, int k) {
-  return and_or(k == 0 ? w << 4 : w >> (4 * (k - 1)), 0x00f000f0u, 0x54005400u);
+// Nibbles k and k + 4 (k = 0..3) of a word as fp16 pairs, code + kBias, into a[k]. Under the exponent of
+// 64 a nibble at mantissa bits 4..7 reads as 64 + c and one at bits 0..3 as 64 + c / 16, which one
+// packed FMA (16 x - 960, exact) turns into 64 + c: that leaves one shift for two nibbles, as the
+// integer pipe, half as wide as the FMA pipe, is the busier one.
+constexpr float kBias = 64.f;
+__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t (&a)[4]) {
+  const __half2 k16 = __float2half2_rn(16.f), k960 = __float2half2_rn(-960.f);
+  auto up = [&](uint32_t x) {
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), k16, k960);
+    return *reinterpret_cast<const uint32_t*>(&r);
+  };
+  const uint32_t t = w >> 8;
+  a[0] = up(and_or(w, 0x000f000fu, 0x54005400u));
+  a[1] = and_or(w, 0x00f000f0u, 0x54005400u);
+  a[2] = up(and_or(t, 0x000f000fu, 0x54005400u));
+  a[3] = and_or(t, 0x00f000f0u, 0x54005400u);
 }
-template <>
-__device__ __forceinline__ uint32_t key_pair<__nv_bfloat16>(uint32_t w, int k) {
-  return and_or(w >> (4 * k), 0x000f000fu, 0x43004300u);
-}
-template <typename T>
-constexpr float kKeyBias = std::is_same<T, __half>::value ? 64.f : 128.f;
-
-// The same of a value word, as fp16 and with a bias of 16.
-__device__ __forceinline__ uint32_t value_pair(uint32_t w, int k) {
-  return and_or(k < 2 ? w << (6 - 4 * k) : w >> (4 * k - 6), 0x03c003c0u, 0x4c004c00u);
-}
-constexpr float kValueBias = 16.f;
+// Values count from the middle code, which keeps the sums of rounded P * scale small.
+constexpr float kMiddle = 8.f;
 // Bits of a scale: infinity, and the mantissa.
 template <typename T>
 constexpr uint32_t kScaleInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
@@ -84,16 +85,39 @@ template <typename T>
 constexpr uint32_t kScaleMantissa = std::is_same<T, __half>::value ? 0x3ffu : 0x7fu;
 constexpr float kValueMiddle = 8.f;
 
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 r;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr));
-  return r;
+// Products, transpositions and shared loads that the compiler may move among one another (those of
+// aeg_common.cuh are volatile and keep their order): a tile's chains overlap only if it does. The
+// loads stay behind the barrier waits, which clobber memory.
+__device__ __forceinline__ void mma_free(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-  uint2 r;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(addr));
-  return r;
+__device__ __forceinline__ uint32_t transpose_free(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
 }
+// Whether the phase with the given parity has completed; does not wait.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// Arrives on `bar` once `value` is known.
+__device__ __forceinline__ void mbar_arrive_after(uint64_t* bar, uint32_t value) {
+  asm volatile("{\n\t.reg .b32 t;\n\tand.b32 t, %1, 0;\n\tadd.u32 t, t, %0;\n\t"
+               "mbarrier.arrive.shared::cta.b64 _, [t];\n\t}" ::"r"(smem_u32(bar)), "r"(value)
+               : "memory");
+}
+__device__ __forceinline__ uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ uint2 lds64(const uint8_t* p) { return *reinterpret_cast<const uint2*>(p); }
 __device__ __forceinline__ void bulk_load_1d_hint(void* smem_dst, const void* gmem_src, uint32_t bytes, uint64_t* bar,
                                                   uint64_t l2_policy) {
   asm volatile(
@@ -103,252 +127,297 @@ __device__ __forceinline__ void bulk_load_1d_hint(void* smem_dst, const void* gm
       : "memory");
 }
 
+// A worker's part of shared memory.
+template <int NT>
+struct Int4Worker {
+  using SL = Int4Smem<NT>;
+  uint8_t* ring;
+  uint8_t* q;
+  uint64_t* full;   // tile landed
+  uint64_t* empty;  // stage free
+  uint64_t* qfull;
+  uint64_t* qempty;
+  int* tokens;      // valid tokens of the stage's tile
+  int4* record;     // {tiles (-1: no more units), partial slot or -1, sequence, KV head}
+  __device__ Int4Worker(uint8_t* smem, int w) {
+    ring = smem + w * SL::kPerWarp;
+    q = ring + SL::kRing;
+    uint8_t* meta = smem + SL::kOffMeta + w * SL::kMeta;
+    full = reinterpret_cast<uint64_t*>(meta);
+    empty = full + SL::kStages;
+    qfull = empty + SL::kStages;
+    qempty = qfull + 1;
+    tokens = reinterpret_cast<int*>(meta + SL::kTokens);
+    record = reinterpret_cast<int4*>(meta + SL::kRecord);
+  }
+};
+
+// The requesting warp: lane w walks worker w's units (their records and queries) and tiles, each
+// step at most one of either. Block ids come two tiles ahead, unit records one unit ahead, so that no
+// step waits for a load it has just made. Without a tensor map there is no zero fill: a tile whose id
+// is outside the pool is not fetched and has no valid tokens.
+template <typename T, int NT>
+__device__ __forceinline__ void request_tiles(const AttnParams& p, uint8_t* smem, int lane) {
+  using SL = Int4Smem<NT>;
+  const uint64_t keep = l2_policy_evict_last(), pol = l2_policy_evict_first();
+  const bool worker = lane < SL::kWarps;
+  const Int4Worker<NT> w(smem, worker ? lane : 0);
+  const int gw = static_cast<int>(blockIdx.x) * SL::kWarps + (worker ? lane : 0);
+
+  int u_beg = 0, u_end = 0, planned_warps = 0, planned_units = 0;
+  int4 ra, rb;
+  auto load_plan = [&]() {
+    u_beg = ld_hint(&p.ws.warp_rec[3 * gw].x, keep);
+    ra = ld_hint(&p.ws.warp_rec[3 * gw + 1], keep);
+    rb = ld_hint(&p.ws.warp_rec[3 * gw + 2], keep);
+    u_end = ld_hint(&p.ws.warp_rec[3 * (gw + 1)].x, keep);
+    planned_warps = ld_hint(&p.ws.header[kHdrWarps], keep);
+    planned_units = ld_hint(&p.ws.header[kHdrUnits], keep);
+  };
+  // The plan and the first tiles come before the wait for the preceding kernel only where the host
+  // knows that it wrote neither.
+  const bool early = p.plan_ready && p.prefetch_kv;
+  if (p.plan_ready) load_plan();
+  if (!early) pdl_wait_primary();
+  if (!p.plan_ready) load_plan();
+  if (!(planned_warps == static_cast<int>(gridDim.x) * SL::kWarps && planned_units <= p.max_units && u_beg >= 0 &&
+        u_beg <= u_end && u_end <= planned_units)) {
+    if (worker && u_beg != u_end) atomicOr(&g_deverr_attn, AEG_DEVERR_PLAN_MISMATCH);
+    u_end = u_beg;
+  }
+
+  // Tiles: unit ut (its record in ra, rb), tile i of n; ids of tiles i and i + 1; the next unit's record.
+  int ut = u_beg, i = 0, n = 0, id0 = 0, id1 = 0, n_ctx = 0;
+  const int* ids = p.tables;
+  const T* tiles = static_cast<const T*>(p.k_cache);
+  int4 na = make_int4(0, 0, 0, -1), nb = make_int4(0, 0, 0, 0);
+  auto enter = [&]() {  // begins unit ut
+    n = ut < u_end ? unit_items(ra, rb, p) : 0;
+    i = 0;
+    if (ut < u_end) {
+      id0 = rb.y;
+      id1 = rb.z;
+      n_ctx = rb.x - ra.y * kBlockTokens;
+      ids = p.tables + static_cast<int64_t>(ra.x / p.Hkv) * p.table_stride + ra.y;
+      tiles = static_cast<const T*>(p.k_cache) + static_cast<int64_t>(ra.x % p.Hkv) * kInt4TileElems;
+      if (ut + 1 < u_end) {
+        na = ld_hint(&p.ws.units[2 * (ut + 1)], keep);
+        nb = ld_hint(&p.ws.units[2 * (ut + 1) + 1], keep);
+      }
+    }
+  };
+  // Queries: unit uq, its record.
+  int uq = u_beg;
+  int4 qa = ra, qb = rb;
+  enter();
+
+  uint32_t st = 0, ph = 1, qph = 1;  // a barrier that has completed no phase counts as free
+  auto tile_step = [&]() -> bool {
+    if (i >= n) {
+      if (ut >= u_end) return false;
+      ++ut;
+      ra = na;
+      rb = nb;
+      enter();
+      return true;
+    }
+    if (!mbar_test(&w.empty[st], ph)) return false;
+    const int id2 = i + 2 < n ? ids[i + 2] : 0;
+    const bool inside = static_cast<uint32_t>(id0) < static_cast<uint32_t>(p.num_blocks);
+    w.tokens[st] = inside ? min(kBlockTokens, n_ctx - i * kBlockTokens) : 0;
+    if (inside) {
+      mbar_arrive_expect_tx(&w.full[st], kInt4TileBytes);
+      bulk_load_1d_hint(w.ring + st * kInt4TileBytes, tiles + static_cast<int64_t>(id0) * p.block_stride, kInt4TileBytes,
+                        &w.full[st], pol);
+    } else {
+      atomicOr(&g_deverr_attn, AEG_DEVERR_BLOCK_ID_RANGE);
+      mbar_arrive(&w.full[st]);
+    }
+    id0 = id1;
+    id1 = id2;
+    ++i;
+    if (++st == SL::kStages) {
+      st = 0;
+      ph ^= 1;
+    }
+    return true;
+  };
+  if (early) {
+    if (worker)
+      for (int k = 0; k < SL::kStages + 2; ++k) tile_step();
+    __syncwarp();
+    pdl_wait_primary();
+  }
+
+  bool run = worker, more_units = worker;
+  uint64_t idle_since = 0;
+  while (__any_sync(0xffffffffu, run)) {
+    bool moved = false;
+    if (run) {
+      if (more_units && mbar_test(w.qempty, qph)) {
+        const int tiles_q = uq < u_end ? unit_items(qa, qb, p) : -1;
+        const int b = qa.x / p.Hkv, h = qa.x % p.Hkv;
+        if (tiles_q == 0) {  // a record that does not fit this call: left out, by the walk over tiles too
+          atomicOr(&g_deverr_attn, AEG_DEVERR_PLAN_MISMATCH);
+        } else {
+          *w.record = make_int4(tiles_q, qa.w, b, h);
+          if (tiles_q > 0 && p.q_bulk) {
+            const uint32_t bytes = p.G * kHeadDim * 2;
+            mbar_arrive_expect_tx(w.qfull, bytes);
+            bulk_load_1d(w.q, static_cast<const T*>(p.q) + static_cast<int64_t>(b) * p.q_stride +
+                                  static_cast<int64_t>(h) * p.G * kHeadDim, bytes, w.qfull);
+          } else {
+            mbar_arrive(w.qfull);
+          }
+          qph ^= 1;
+        }
+        more_units = tiles_q >= 0;
+        ++uq;
+        if (uq < u_end) {
+          qa = ld_hint(&p.ws.units[2 * uq], keep);
+          qb = ld_hint(&p.ws.units[2 * uq + 1], keep);
+        }
+        moved = true;
+      }
+      if (tile_step()) moved = true;
+      run = more_units || ut < u_end;
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+      idle_since = 0;
+    } else {
+      const uint64_t now = globaltimer_ns();
+      if (idle_since == 0) idle_since = now;
+      if (now - idle_since > kWaitLimitNs) {
+        if (lane == 0) atomicOr(&g_deverr_attn, AEG_DEVERR_WAIT_TIMEOUT);
+        return;
+      }
+      __nanosleep(40);
+    }
+  }
+}
+
 template <typename T, int NT>
 __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_kernel(const AttnParams p) {
   using SL = Int4Smem<NT>;
-  constexpr int kW = SL::kWarps, kSt = SL::kStages, kBatch = SL::kBatch;
-  constexpr float kNoMax = -1e30f;     // the running maximum before the first score
-  constexpr float kSlack = 6.f;        // scores may exceed the running maximum by this (log2 units)
-  constexpr float kTop = 512.f;        // largest scaled scale: 2^9 * 2^kSlack = 2^15 fits fp16
-  constexpr int kFold = 32;            // tiles between two removals of the constant from O
+  constexpr int kW = SL::kWarps, kSt = SL::kStages;
+  constexpr float kNoMax = -1e30f;  // the running maximum before the first score
+  constexpr float kSlack = 6.f;     // scores may exceed the running maximum by this (log2 units)
+  constexpr float kTop = 512.f;     // largest scaled scale: 2^9 * 2^kSlack = 2^15 fits fp16
+  constexpr int kFold = 16;         // tiles between two removals of the constant from O
   const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 127) & ~127u) - raw);
-
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  uint8_t* ring = smem + warp * SL::kPerWarp;
-  T* qslot = reinterpret_cast<T*>(ring + kSt * kInt4TileBytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + SL::kOffBars) + warp * SL::kBarsPerWarp;
-  uint64_t* qbar = full + kSt;
-  uint32_t* qdep_slot = reinterpret_cast<uint32_t*>(full + kSt + 1);
 
-  if (lane == 0) {
-    for (int s = 0; s < kSt; ++s) mbar_init(&full[s], 1);
-    mbar_init(qbar, 1);
+  if (warp < kW && lane == 0) {
+    const Int4Worker<NT> w(smem, warp);
+    for (int s = 0; s < SL::kBars; ++s) mbar_init(&w.full[s], 1);
     fence_mbar_init();
   }
-  __syncwarp();
-
-  // Plan records, as in decode_attn_kernel.
-  const int gw = static_cast<int>(blockIdx.x) * kW + warp;
-  const uint64_t keep = l2_policy_evict_last();
-  int4 r0 = make_int4(0, 0, 0, 0);
-  auto load_plan = [&]() {
-    if (lane < 3)
-      r0 = ld_hint(&p.ws.warp_rec[3 * gw + lane], keep);
-    else if (lane == 3)
-      r0.x = ld_hint(&p.ws.warp_rec[3 * (gw + 1)].x, keep);
-    else if (lane == 4)
-      r0.x = ld_hint(&p.ws.header[kHdrWarps], keep);
-    else if (lane == 5)
-      r0.x = ld_hint(&p.ws.header[kHdrUnits], keep);
-    else if (lane == 6)
-      r0.x = ld_hint(&p.ws.header[kHdrSplitPairs], keep);
-    else if (lane == 7)
-      r0 = ld_hint(&p.ws.merge_rec[gw], keep);
-  };
-  if (p.plan_ready) load_plan();
-  const bool early = p.plan_ready && p.prefetch_kv;
-  if (!early) {
-    pdl_wait_primary();
-    pdl_launch_dependents();
-    if (!p.plan_ready) load_plan();
+  __syncthreads();
+  if (warp == kW) {
+    request_tiles<T, NT>(p, smem, lane);
+    return;
   }
 
+  const Int4Worker<NT> wk(smem, warp);
+  const uint8_t* const ring = wk.ring;
+  const int gw = static_cast<int>(blockIdx.x) * kW + warp;
   const int G = p.G;
-  const int Hkv = p.Hkv;
   const int total_warps = static_cast<int>(gridDim.x) * kW;
-  const uint64_t pol = l2_policy_evict_first();
-  const T* q = static_cast<const T*>(p.q);
+  const uint64_t keep = l2_policy_evict_last();
   T* out = static_cast<T*>(p.out);
   const int quad = lane & 3;  // column pair of the accumulator fragment
   const int grp = lane >> 2;  // row of the accumulator fragment
+  pdl_wait_primary();
+  pdl_launch_dependents();
 
-  bool abort = false;
-  uint32_t g_iss = 0, g_con = 0;      // tiles requested / consumed by this warp
-  uint32_t st_iss = 0, st_con = 0;    // their stages
-  uint32_t ph_con = 0;
-  const float sc = fmaxf(fabsf(p.scale_log2), 1e-30f);  // not 0, so that -infinity stays below all scores
-  const float slack = kSlack / sc;
-  uint32_t bad = 0;                   // stages whose block id was outside the pool
-  uint32_t q_phase = 0;
+  // This warp's share of the split merge and the launches with this plan so far (see
+  // decode_attn_kernel); needed when its units are done.
+  int4 mr = make_int4(0, 0, 0, 0);
+  if (lane == 0) mr = ld_hint(&p.ws.merge_rec[gw], keep);
+  else if (lane == 1) mr.x = ld_hint(&p.ws.header[kHdrWarps], keep);
+  else if (lane == 2) mr.x = ld_hint(&p.ws.header[kHdrSplitPairs], keep);
+  else if (lane == 3) mr.x = ld_relaxed_gpu(&p.ws.warp_flag[gw * kFlagStride]);
 
-  auto report_timeout = [&]() {
-    abort = true;
-    if (lane == 0) atomicOr(&g_deverr_attn, AEG_DEVERR_WAIT_TIMEOUT);
-  };
-
-  const int u_beg = __shfl_sync(0xffffffffu, r0.x, 0);
-  const int u_end = __shfl_sync(0xffffffffu, r0.x, 3);
-  const int planned_warps = __shfl_sync(0xffffffffu, r0.x, 4);
-  const int planned_units = __shfl_sync(0xffffffffu, r0.x, 5);
-  const int n_entries = min(max(__shfl_sync(0xffffffffu, r0.x, 6), 0), p.num_pairs);
-  const int4 mr = shfl4(r0, 7);
-  int n_units = u_end - u_beg;
-  if (!(planned_warps == total_warps && planned_units <= p.max_units && u_beg >= 0 && u_beg <= u_end &&
-        u_end <= planned_units)) {
-    if (lane == 0 && n_units != 0) atomicOr(&g_deverr_attn, AEG_DEVERR_PLAN_MISMATCH);
-    n_units = 0;
-  }
-
-  // Unit records, one per lane: lane (k % 32) holds the worker's unit k for the 32 units from the
-  // one being computed on. Lane 0 takes unit 0 from the start record.
-  int4 ra = shfl4(r0, 1), rb = shfl4(r0, 2);
-  if (lane > 0) {
-    if (lane < n_units) {
-      ra = ld_hint(&p.ws.units[2 * (u_beg + lane)], keep);
-      rb = ld_hint(&p.ws.units[2 * (u_beg + lane) + 1], keep);
-    } else {
-      ra = make_int4(0, 0, 0, -1);
-      rb = make_int4(0, 0, 0, 0);
-    }
-  }
-
-  auto load_q = [&](int k) {
-    const int4 a = shfl4(ra, k & 31), bb = shfl4(rb, k & 31);
-    if (unit_items(a, bb, p) == 0) {
-      if (lane == 0) mbar_arrive(qbar);
-      return;
-    }
-    const int b = a.x / Hkv, h = a.x % Hkv;
-    const T* qsrc = q + static_cast<int64_t>(b) * p.q_stride + static_cast<int64_t>(h) * G * kHeadDim;
-    const uint32_t qbytes = G * kHeadDim * 2;
-    if (p.q_bulk) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(qbar, qbytes);
-        bulk_load_1d(qslot, qsrc, qbytes, qbar);
-      }
-    } else {
-      for (int i = lane; i < G * kHeadDim / 2; i += 32)
-        reinterpret_cast<uint32_t*>(qslot)[i] = reinterpret_cast<const uint32_t*>(qsrc)[i];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(qbar);
+  bool lost = false;  // a wait ran out: this warp's results are not complete
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return;
+    if (lost || !mbar_wait_bounded(bar, parity, kWaitLimitNs)) {
+      if (!lost && lane == 0) atomicOr(&g_deverr_attn, AEG_DEVERR_WAIT_TIMEOUT);
+      lost = true;
     }
   };
+  uint32_t st_con = 0, ph_con = 0, q_phase = 0;
 
-  // Issue walker: requests the worker's tiles in order, one lane a tile. Block ids of items 0..2 of
-  // a unit come with its record (lanes 0..2), later ones from a 32-entry chunk of the block table
-  // loaded when the walker enters the unit (the chunk after it one chunk ahead).
-  int ik = -1, ii = 0, in_ = 0, irec = 0, itbase = 3, itbl = 0, itnext = 0;
-  const int* itab = p.tables;
-  const T* ihead = static_cast<const T*>(p.k_cache);
-  auto issue_enter = [&](int k) {
-    ik = k;
-    ii = 0;
-    in_ = 0;
-    if (k >= n_units) return;
-    const int4 a = shfl4(ra, k & 31), bb = shfl4(rb, k & 31);
-    in_ = unit_items(a, bb, p);
-    if (in_ == 0) return;
-    ihead = static_cast<const T*>(p.k_cache) + static_cast<int64_t>(a.x % Hkv) * kInt4TileElems;
-    irec = lane == 0 ? bb.y : (lane == 1 ? bb.z : bb.w);
-    itab = p.tables + static_cast<int64_t>(a.x / Hkv) * p.table_stride + a.y;
-    itbase = 3;
-    itbl = lane < in_ - 3 ? itab[3 + lane] : 0;
-    itnext = lane < in_ - 35 ? itab[35 + lane] : 0;
-  };
-  auto refill = [&]() {
-    int room = kSt - static_cast<int>(g_iss - g_con);
-    while (room > 0) {
-      if (ii >= in_) {
-        if (ik >= n_units) break;
-        issue_enter(ik + 1);
-        continue;
-      }
-      int first, left, blk;
-      const bool from_rec = ii < 3;
-      if (from_rec) {
-        first = ii;
-        left = min(in_, 3) - ii;
-        blk = irec;
-      } else {
-        if (ii - itbase >= 32) {
-          itbase += 32;
-          itbl = itnext;
-          itnext = lane < in_ - itbase - 32 ? itab[itbase + 32 + lane] : 0;
-        }
-        first = ii - itbase;
-        left = min(in_, itbase + 32) - ii;
-        blk = itbl;
-      }
-      const int cnt = min(left, room);
-      const int r = lane - first;  // this lane's tile of the batch
-      const bool mine = r >= 0 && r < cnt;
-      const bool inside = static_cast<uint32_t>(blk) < static_cast<uint32_t>(p.num_blocks);
-      uint32_t st = st_iss + static_cast<uint32_t>(r);
-      st = st >= kSt ? st - kSt : st;
-      if (mine && !abort) {
-        if (inside) {
-          mbar_arrive_expect_tx(&full[st], kInt4TileBytes);
-          bulk_load_1d_hint(ring + st * kInt4TileBytes, ihead + static_cast<int64_t>(blk) * p.block_stride, kInt4TileBytes,
-                            &full[st], pol);
-        } else {
-          atomicOr(&g_deverr_attn, AEG_DEVERR_BLOCK_ID_RANGE);
-          mbar_arrive(&full[st]);
-        }
-      }
-      const uint32_t out_of_pool = __ballot_sync(0xffffffffu, mine && !inside);
-      if (out_of_pool | bad) {
-        for (int j = 0; j < cnt; ++j) {
-          const uint32_t sj = (st_iss + j) % kSt;
-          bad = (bad & ~(1u << sj)) | (((out_of_pool >> (first + j)) & 1u) << sj);
-        }
-      }
-      g_iss += cnt;
-      st_iss = st_iss + cnt >= kSt ? st_iss + cnt - kSt : st_iss + cnt;
-      ii += cnt;
-      // The chunk requested on entering the unit may still be on its way: later items wait for the
-      // next call, unless nothing else is in the ring.
-      room = from_rec && g_iss - g_con >= 3 ? 0 : room - cnt;
-    }
-  };
-
-  if (early) {
-    refill();
-    pdl_wait_primary();
-    pdl_launch_dependents();
-  }
-  if (n_units > 0) load_q(0);
-  refill();
-  const int epoch_word = lane == 0 ? ld_relaxed_gpu(&p.ws.warp_flag[gw * kFlagStride]) : 0;
-
-  for (int c = 0; c < n_units; ++c) {
-    if (c > 0 && lane == ((c - 1) & 31) && c + 31 < n_units) {
-      ra = p.ws.units[2 * (u_beg + c + 31)];
-      rb = p.ws.units[2 * (u_beg + c + 31) + 1];
-    }
-    const int4 ua = shfl4(ra, c & 31), ub = shfl4(rb, c & 31);
-    const int n = unit_items(ua, ub, p);
-    if (n == 0 && lane == 0) atomicOr(&g_deverr_attn, AEG_DEVERR_PLAN_MISMATCH);
-    const int b = ua.x / Hkv, h = ua.x % Hkv, j0 = ua.y, slot = ua.w, n_ctx = ub.x;
-
-    if (!abort && !mbar_wait_bounded(qbar, q_phase, kWaitLimitNs)) report_timeout();
+  while (!lost) {
+    wait(wk.qfull, q_phase);
+    if (lost) break;
     q_phase ^= 1;
-    // Query fragments: contraction step 2 w + u pairs dims (d, d + 4) and (d + 1, d + 5) with
-    // d = 32 w + 8 quad + 2 u, as the code words do. Then the sums of q over each group, for the
-    // fragment's two columns.
-    // A negative scale goes into the sign of q, so that larger sums always mean larger scores.
+    const int4 rec = *wk.record;
+    const int n = rec.x, slot = rec.y, b = rec.z, h = rec.w;
+    if (n < 0) break;
+
+    // A negative scale goes into the sign of q, so that larger sums always mean larger scores. bf16
+    // queries go to fp16 exactly after a power of two of the head's own (elements below 2^-17 of the
+    // head's largest are rounded at 2^-24 of it), which returns with the scale of the scores.
     const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
     uint32_t qf[NT][8][2];
     float qs[NT][2][2];  // [column][group]
+    float sc[NT][2];     // scores to log2 units [column]
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int head = nt * 8 + grp;
-      float sum[2] = {0.f, 0.f};
+      uint32_t xw[4][4];
+      uint32_t top = 0;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (head < G) x = lds128(smem_u32(qslot) + head * (kHeadDim * 2) + w * 64 + quad * 16);
-        x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
-        qf[nt][2 * w][0] = __byte_perm(x.x, x.z, 0x5410);
-        qf[nt][2 * w][1] = __byte_perm(x.x, x.z, 0x7632);
-        qf[nt][2 * w + 1][0] = __byte_perm(x.y, x.w, 0x5410);
-        qf[nt][2 * w + 1][1] = __byte_perm(x.y, x.w, 0x7632);
-        const float2 f0 = unpack2<T>(x.x), f1 = unpack2<T>(x.y), f2 = unpack2<T>(x.z), f3 = unpack2<T>(x.w);
-        sum[w >> 1] += ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
+        if (head < G && p.q_bulk) {
+          x = lds128(wk.q + head * (kHeadDim * 2) + w * 64 + quad * 16);
+        } else if (head < G) {  // rows that are not 16-byte aligned
+          const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + static_cast<int64_t>(b) * p.q_stride +
+                                                                  (static_cast<int64_t>(h) * G + head) * kHeadDim + w * 32 + quad * 8);
+          x = make_uint4(src[0], src[1], src[2], src[3]);
+        }
+        xw[w][0] = x.x ^ flip;
+        xw[w][1] = x.y ^ flip;
+        xw[w][2] = x.z ^ flip;
+        xw[w][3] = x.w ^ flip;
+        if constexpr (!std::is_same<T, __half>::value)
+          for (int i = 0; i < 4; ++i) top = __vmaxu2(top, xw[w][i] & 0x7fff7fffu);
+      }
+      float back = 1.f;
+      if constexpr (!std::is_same<T, __half>::value) {
+        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = static_cast<int>(max(top & 0xffffu, top >> 16) >> 7);  // exponent of the largest |q|
+        const int ef = min(max(254 - e, 1), 253);
+        const float to = __uint_as_float(static_cast<uint32_t>(ef) << 23);  // 2^(127 - e): |q| below 2
+        back = __uint_as_float(static_cast<uint32_t>(254 - ef) << 23);
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack2<T>(xw[w][i]);
+            xw[w][i] = pack2<__half>(f.x * to, f.y * to);
+          }
+      }
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        qf[nt][2 * w][0] = __byte_perm(xw[w][0], xw[w][2], 0x5410);
+        qf[nt][2 * w][1] = __byte_perm(xw[w][0], xw[w][2], 0x7632);
+        qf[nt][2 * w + 1][0] = __byte_perm(xw[w][1], xw[w][3], 0x5410);
+        qf[nt][2 * w + 1][1] = __byte_perm(xw[w][1], xw[w][3], 0x7632);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = unpack2<__half>(xw[w][i]);
+          sum[w >> 1] += f.x + f.y;
+        }
       }
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
@@ -357,19 +426,21 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
         qs[nt][0][g] = __shfl_sync(0xffffffffu, sum[g], 8 * quad);
         qs[nt][1][g] = __shfl_sync(0xffffffffu, sum[g], 8 * quad + 4);
       }
+      // Not 0, so that -infinity stays below all scores.
+      back = fmaxf(back * fabsf(p.scale_log2), 1e-37f);
+      sc[nt][0] = __shfl_sync(0xffffffffu, back, 8 * quad);
+      sc[nt][1] = __shfl_sync(0xffffffffu, back, 8 * quad + 4);
     }
-    // The next unit's rows overwrite the slot: make every lane's slot reads complete first.
+    // The slot is free once every lane's values have arrived: a vote on them needs them all.
     {
       uint32_t dep = 0;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) dep ^= qf[nt][ks][0] ^ qf[nt][ks][1];
-      if (lane == 0) *qdep_slot = dep;
+        for (int ks = 0; ks < 8; ++ks) dep |= qf[nt][ks][0] | qf[nt][ks][1];
+      const uint32_t any = __ballot_sync(0xffffffffu, dep != 0);
+      if (lane == 0) mbar_arrive_after(wk.qempty, any);
     }
-    __syncwarp();
-    if (c + 1 < n_units) load_q(c + 1);
-    if (n == 0) continue;
 
     // Running maximum of the unscaled scores, that times the scale, and the score from which it moves;
     // sum of p; sum of p * (minimum + middle * scale) [column][group]; sum of the rounded P * scale
@@ -383,8 +454,8 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         m[nt][i] = kNoMax;
-        ms[nt][i] = kNoMax * sc;
-        mt_[nt][i] = kNoMax + slack;
+        ms[nt][i] = kNoMax * sc[nt][i];
+        mt_[nt][i] = kNoMax + kSlack / sc[nt][i];
         l[nt][i] = om[nt][i][0] = om[nt][i][1] = 0.f;
         ps[i][nt][0] = ps[i][nt][1] = ps[i][nt][2] = ps[i][nt][3] = 0.f;
       }
@@ -400,15 +471,15 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
 #pragma unroll
           for (int mt = 4 * g; mt < 4 * g + 4; ++mt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[mt][nt][i] = fmaf(-(kValueBias + kValueMiddle), ps[g][nt][i], o[mt][nt][i]);
+            for (int i = 0; i < 4; ++i) o[mt][nt][i] = fmaf(-(kBias + kMiddle), ps[g][nt][i], o[mt][nt][i]);
           ps[g][nt][0] = ps[g][nt][1] = ps[g][nt][2] = ps[g][nt][3] = 0.f;
         }
     };
 
     // Scores of the tile in stage `st`, unscaled: S^T, one accumulator per group; rows are tokens grp
     // and grp + 8.
-    auto scores = [&](uint32_t st, float (&x)[NT][4]) {
-      const uint32_t tile = smem_u32(ring) + st * kInt4TileBytes;
+    auto scores = [&](uint32_t st, float (*x)[4]) {
+      const uint8_t* tile = ring + st * kInt4TileBytes;
       const uint4 kc0 = lds128(tile + grp * 64 + quad * 16), kc1 = lds128(tile + 512 + grp * 64 + quad * 16);
       const uint2 kp0 = lds64(tile + kInt4KeyPairs + grp * 8), kp1 = lds64(tile + kInt4KeyPairs + 64 + grp * 8);
       const uint32_t kw0[4] = {kc0.x, kc0.y, kc0.z, kc0.w}, kw1[4] = {kc1.x, kc1.y, kc1.z, kc1.w};
@@ -418,16 +489,19 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
-        for (int w = 2 * g; w < 2 * g + 2; ++w)
+        for (int w = 2 * g; w < 2 * g + 2; ++w) {
+          uint32_t lo[4], hi[4];
+          code_pairs(kw0[w], lo);
+          code_pairs(kw1[w], hi);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const uint32_t a[4] = {key_pair<T>(kw0[w], 2 * u), key_pair<T>(kw1[w], 2 * u), key_pair<T>(kw0[w], 2 * u + 1),
-                                   key_pair<T>(kw1[w], 2 * u + 1)};
+            const uint32_t a[4] = {lo[2 * u], hi[2 * u], lo[2 * u + 1], hi[2 * u + 1]};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) MmaF32<T>::run(s[nt], a, qf[nt][2 * w + u][0], qf[nt][2 * w + u][1]);
+            for (int nt = 0; nt < NT; ++nt) mma_free(s[nt], a, qf[nt][2 * w + u][0], qf[nt][2 * w + u][1]);
           }
+        }
         const float2 f0 = unpack2<T>(g == 0 ? kp0.x : kp0.y), f1 = unpack2<T>(g == 0 ? kp1.x : kp1.y);
-        const float b0 = fmaf(-kKeyBias<T>, f0.x, f0.y), b1 = fmaf(-kKeyBias<T>, f1.x, f1.y);
+        const float b0 = fmaf(-kBias, f0.x, f0.y), b1 = fmaf(-kBias, f1.x, f1.y);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -440,7 +514,7 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
 
     // Makes room for the scores x and the scales under vtop: the maxima move to the tile's, and what
     // was summed so far follows.
-    auto make_room = [&](const float (&x)[NT][4], uint32_t vtop) {
+    auto make_room = [&](const float (*x)[4], uint32_t vtop) {
       uint32_t top = vtop;
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
@@ -462,10 +536,10 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
           float mx = fmaxf(x[nt][i], x[nt][i + 2]);
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-          const float mn = fmaxf(m[nt][i], mx), a = ex2((m[nt][i] - mn) * sc);
+          const float mn = fmaxf(m[nt][i], mx), a = ex2((m[nt][i] - mn) * sc[nt][i]);
           m[nt][i] = mn;
-          ms[nt][i] = mn * sc;
-          mt_[nt][i] = mn + slack;
+          ms[nt][i] = mn * sc[nt][i];
+          mt_[nt][i] = mn + kSlack / sc[nt][i];
           l[nt][i] *= a;
           om[nt][i][0] *= a;
           om[nt][i][1] *= a;
@@ -482,15 +556,16 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
         }
     };
 
-    // Adds the tile in stage `st` with scores x. Tokens from nvalid on get no weight and, whatever their
+    // Adds the tile in stage `st` with scores x. Tokens from `valid` on get no weight and, whatever their
     // value pairs hold, count as zeros. With kNext the next tile's scores are made on the way: their
     // chain of MMAs runs beside this tile's exponents and products.
-    auto add_tile = [&](auto next_tag, uint32_t st, uint32_t st_next, float (&x)[NT][4], float (&x_next)[NT][4], int nvalid) {
+    auto add_tile = [&](auto next_tag, uint32_t st, uint32_t st_next, float (*x)[4], float (*x_next)[4]) {
       constexpr bool kNext = decltype(next_tag)::value;
-      const uint32_t tile = smem_u32(ring) + st * kInt4TileBytes;
+      const uint8_t* tile = ring + st * kInt4TileBytes;
+      const int valid = wk.tokens[st];
       uint2 vp0 = lds64(tile + kInt4ValuePairs + grp * 8), vp1 = lds64(tile + kInt4ValuePairs + 64 + grp * 8);
-      if (!kNext && nvalid < kBlockTokens) {  // only a sequence's last tile is partly filled
-        const bool in0 = grp < nvalid, in1 = grp + 8 < nvalid;
+      if (valid < kBlockTokens) {
+        const bool in0 = grp < valid, in1 = grp + 8 < valid;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           if (!in0) x[nt][0] = x[nt][1] = -INFINITY;
@@ -504,81 +579,80 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
       bool over = vtop > vlim;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
-        over = over || fmaxf(x[nt][0], x[nt][2]) > mt_[nt][0] || fmaxf(x[nt][1], x[nt][3]) > mt_[nt][1];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) over = over || fmaxf(x[nt][i], x[nt][i + 2]) > mt_[nt][i];
       if (__any_sync(0xffffffffu, over)) make_room(x, vtop);
 
       if constexpr (kNext) scores(st_next, x_next);
-      const uint4 vc0 = lds128(tile + kInt4ValueCodes + quad * 128 + grp * 16);
-      const uint4 vc1 = lds128(tile + kInt4ValueCodes + 512 + quad * 128 + grp * 16);
+      const uint8_t* vcodes = tile + kInt4ValueCodes + quad * 128 + grp * 16;
+      const uint4 vc0 = lds128(vcodes), vc1 = lds128(vcodes + 512);
 
       // P, its sums, and P * scale of each group, turned around in registers.
       uint32_t pv[2][NT][2];
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const float2 f0 = unpack2<T>(g == 0 ? vp0.x : vp0.y), f1 = unpack2<T>(g == 0 ? vp1.x : vp1.y);
-        const float b0 = fmaf(kValueMiddle, f0.x, f0.y), b1 = fmaf(kValueMiddle, f1.x, f1.y);
+        const float b0 = fmaf(kMiddle, f0.x, f0.y), b1 = fmaf(kMiddle, f1.x, f1.y);
         const float s0 = f0.x * vmul, s1 = f1.x * vmul;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+          float* p_ = x[nt];
           if (g == 0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[nt][i] = ex2(fmaf(x[nt][i], sc, -ms[nt][i & 1]));
-            l[nt][0] += x[nt][0] + x[nt][2];
-            l[nt][1] += x[nt][1] + x[nt][3];
+            for (int i = 0; i < 4; ++i) p_[i] = ex2(fmaf(p_[i], sc[nt][i & 1], -ms[nt][i & 1]));
+            l[nt][0] += p_[0] + p_[2];
+            l[nt][1] += p_[1] + p_[3];
           }
-          om[nt][0][g] = fmaf(x[nt][0], b0, fmaf(x[nt][2], b1, om[nt][0][g]));
-          om[nt][1][g] = fmaf(x[nt][1], b0, fmaf(x[nt][3], b1, om[nt][1][g]));
-          pv[g][nt][0] = movmatrix_trans(pack2<__half>(x[nt][0] * s0, x[nt][1] * s0));
-          pv[g][nt][1] = movmatrix_trans(pack2<__half>(x[nt][2] * s1, x[nt][3] * s1));
-          MmaF32<__half>::run(ps[g][nt], ones, pv[g][nt][0], pv[g][nt][1]);
+          om[nt][0][g] = fmaf(p_[0], b0, fmaf(p_[2], b1, om[nt][0][g]));
+          om[nt][1][g] = fmaf(p_[1], b0, fmaf(p_[3], b1, om[nt][1][g]));
+          pv[g][nt][0] = transpose_free(pack2<__half>(p_[0] * s0, p_[1] * s0));
+          pv[g][nt][1] = transpose_free(pack2<__half>(p_[2] * s1, p_[3] * s1));
+          mma_free(ps[g][nt], ones, pv[g][nt][0], pv[g][nt][1]);
         }
       }
 
       // O^T: row grp of tile mt is dim 64 (mt / 4) + 8 grp + 2 (mt % 4), row grp + 8 the next dim.
       const uint32_t vw0[4] = {vc0.x, vc0.y, vc0.z, vc0.w}, vw1[4] = {vc1.x, vc1.y, vc1.z, vc1.w};
 #pragma unroll
-      for (int mt = 0; mt < 8; ++mt) {
-        const int w = mt >> 1, u = 2 * (mt & 1);
-        const uint32_t a[4] = {value_pair(vw0[w], u), value_pair(vw0[w], u + 1), value_pair(vw1[w], u),
-                               value_pair(vw1[w], u + 1)};
+      for (int w = 0; w < 4; ++w) {
+        uint32_t lo[4], hi[4];
+        code_pairs(vw0[w], lo);
+        code_pairs(vw1[w], hi);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) MmaF32<__half>::run(o[mt][nt], a, pv[mt >> 2][nt][0], pv[mt >> 2][nt][1]);
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t a[4] = {lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1]};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_free(o[2 * w + j][nt], a, pv[w >> 1][nt][0], pv[w >> 1][nt][1]);
+        }
       }
     };
 
-    // The unit's tiles. A tile that is not computed (an id outside the pool) breaks the chain of scores
-    // made ahead.
     float x[NT][4], x_next[NT][4];
-    bool have = false;  // x holds the scores of the tile in stage st_con, which has landed
+    wait(&wk.full[st_con], ph_con);
+    if (lost) break;
+    scores(st_con, x);
     for (int k = 0; k < n; ++k) {
-      if (!have && !abort && !mbar_wait_bounded(&full[st_con], ph_con, kWaitLimitNs)) report_timeout();
-      const uint32_t st_next = st_con + 1 == kSt ? 0 : st_con + 1;
-      const uint32_t ph_next = st_con + 1 == kSt ? ph_con ^ 1 : ph_con;
-      const int nvalid = min(kBlockTokens, n_ctx - (j0 + k) * kBlockTokens);
-      const bool use = !abort && nvalid > 0 && !((bad >> st_con) & 1u);
-      if (use && !have) scores(st_con, x);
-      have = false;
-      if (k + 1 < n && use && !((bad >> st_next) & 1u)) {
-        if (!mbar_wait_bounded(&full[st_next], ph_next, kWaitLimitNs)) {
-          report_timeout();
-        } else {
-          add_tile(std::true_type{}, st_con, st_next, x, x_next, kBlockTokens);
-          have = true;
-        }
-      } else if (use) {
-        add_tile(std::false_type{}, st_con, st_next, x, x_next, nvalid);
+      const bool wraps = st_con + 1 == kSt;
+      const uint32_t st_next = wraps ? 0 : st_con + 1, ph_next = wraps ? ph_con ^ 1 : ph_con;
+      if (k + 1 < n) {
+        wait(&wk.full[st_next], ph_next);
+        if (lost) break;
+        add_tile(std::true_type{}, st_con, st_next, x, x_next);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[nt][i] = x_next[nt][i];
+      } else {
+        add_tile(std::false_type{}, st_con, st_next, x, x_next);
       }
       if ((k & (kFold - 1)) == kFold - 1) fold();
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[nt][i] = x_next[nt][i];
+      // Every lane's reads of the stage have fed its products.
       __syncwarp();
-      ++g_con;
+      if (lane == 0) mbar_arrive(&wk.empty[st_con]);
       st_con = st_next;
       ph_con = ph_next;
-      if (kSt - static_cast<int>(g_iss - g_con) >= kBatch || k + 1 == n) refill();
     }
+    if (lost) break;
 
     // ---- unit result: sums over the tokens of all rows, then 8 consecutive dims a group and lane ----
 #pragma unroll
@@ -631,17 +705,19 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
   }
 
   // Publication and split merge, as in decode_attn_kernel.
-  int entry = mr.x, k = mr.y;
-  const bool share_ok = planned_warps == total_warps && mr.z >= 0 && entry >= 0 && entry <= n_entries;
+  const int planned_warps = __shfl_sync(0xffffffffu, mr.x, 1);
+  const int n_entries = min(max(__shfl_sync(0xffffffffu, mr.x, 2), 0), p.num_pairs);
+  const int stamp = static_cast<int>(static_cast<unsigned>(__shfl_sync(0xffffffffu, mr.x, 3)) + 1u);  // this launch's
+  const int4 share = shfl4(mr, 0);
+  int entry = share.x, k = share.y;
+  const bool share_ok = planned_warps == total_warps && share.z >= 0 && entry >= 0 && entry <= n_entries;
   const int4 none = make_int4(-1, 0, (1 | (1 << 8)) << 16, 0);
-  int4 me = (share_ok && mr.z > 0 && entry < n_entries) ? p.ws.split_pairs[entry] : none;
-  const int epoch = __shfl_sync(0xffffffffu, epoch_word, 0);
-  const int stamp = static_cast<int>(static_cast<unsigned>(epoch) + 1u);
+  int4 me = (share_ok && share.z > 0 && entry < n_entries) ? p.ws.split_pairs[entry] : none;
   __syncwarp();
   if (lane == 0) st_release_gpu(&p.ws.warp_flag[gw * kFlagStride], stamp);
   int ready_entry = -1;
   if (share_ok) {
-    for (int left = mr.z; left > 0; --left) {
+    for (int left = share.z; left > 0; --left) {
       if (k >= merge_items(me.z >> 16, G)) {
         ++entry;
         k = 0;

@@ -32,8 +32,42 @@ def _stream(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _launch(index: int, what: str, fn, *args) -> None:
+    """Calls ``fn(*args, stream)`` with device ``index`` current, on its current stream. A decode step is
+    dozens of such calls: the device is switched only when it has to be."""
+    if torch.cuda.current_device() == index:
+        st = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            st = fn(*args, _raw_stream(index))
+    if st:
+        check(st, what)
+
+
+def _on_device(index: int, t: torch.Tensor, name: str) -> None:
+    """Raises ValueError unless ``t`` is a tensor on CUDA device ``index``, where the work runs."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != index:
+        _require_cuda(t, name)
+        raise ValueError(f"{name} is on {t.device}, the operation runs on cuda:{index}")
+
+
+def _token_rows(t: torch.Tensor, name: str, what: str) -> torch.Size:
+    """The shape of a CUDA ``[tokens, heads, head_dim]`` tensor whose heads are contiguous."""
+    _require_cuda(t, name)
+    shape = t.shape
+    if len(shape) == 3:
+        stride = t.stride()
+        if stride[2] == 1 and stride[1] == shape[2]:
+            return shape
+    raise ValueError(f"{name} must be {what} with contiguous heads")
+
+
 def _require_cuda(t: torch.Tensor, name: str) -> None:
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
 
 
@@ -541,34 +575,44 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Te
 # 4-bit KV cache (layout.int4_block_shape): write and read-back
 
 
-def _int4_layer(kv_cache: torch.Tensor, layer: int, heads: int | None = None) -> int:
-    """Checks a 4-bit cache (and its KV head count) and returns the address of ``layer``'s first tile."""
+def _int4_layer(kv_cache: torch.Tensor, layer: int) -> tuple[int, int, int, int]:
+    """Checks a 4-bit cache; returns the address of ``layer``'s first tile, the elements between blocks,
+    the blocks and the KV heads."""
     _require_cuda(kv_cache, "kv_cache")
-    if kv_cache.dim() != 4 or kv_cache.size(3) != INT4_TILE or kv_cache.dtype not in _DTYPES:
+    shape = kv_cache.shape
+    if len(shape) != 4 or shape[3] != INT4_TILE or kv_cache.dtype not in _DTYPES:
         raise ValueError(f"kv_cache must be a 4-bit cache (N, L, Hkv, {INT4_TILE}) of fp16 or bf16, got "
-                         f"{tuple(kv_cache.shape)} of {kv_cache.dtype}")
+                         f"{tuple(shape)} of {kv_cache.dtype}")
     if not kv_cache.is_contiguous():
         raise ValueError("kv_cache must be contiguous")
-    if heads is not None and kv_cache.size(2) != heads:
-        raise ValueError(f"kv_cache holds {kv_cache.size(2)} KV heads, not {heads}")
-    if not 0 <= layer < kv_cache.size(1):
-        raise ValueError(f"layer {layer} outside [0, {kv_cache.size(1)})")
-    return kv_cache.data_ptr() + layer * kv_cache.size(2) * INT4_TILE * 2
+    N, L, Hkv, _ = shape
+    if not 0 <= layer < L:
+        raise ValueError(f"layer {layer} outside [0, {L})")
+    return kv_cache.data_ptr() + layer * Hkv * INT4_TILE * 2, L * Hkv * INT4_TILE, N, Hkv
 
 
-def _int4_rows(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:
-    for name, t in (("key", key), ("value", value)):
-        _require_cuda(t, name)
-        if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.size(2):
-            raise ValueError(f"{name} must be [T, Hkv, D] with contiguous heads")
-        if t.dtype != kv_cache.dtype:
-            raise ValueError(f"{name} dtype {t.dtype} differs from cache dtype {kv_cache.dtype}")
-    if key.shape != value.shape:
+def _int4_move(fn, what: str, key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, layer: int,
+               slot_mapping: torch.Tensor) -> None:
+    base, block_stride, N, Hkv = _int4_layer(kv_cache, layer)
+    shape = _token_rows(key, "key", "[T, Hkv, D]")
+    if _token_rows(value, "value", "[T, Hkv, D]") != shape:
         raise ValueError("key and value must have the same shape")
+    T, heads, D = shape
+    dtype = kv_cache.dtype
+    if key.dtype != dtype or value.dtype != dtype:
+        raise ValueError(f"key dtype {key.dtype} or value dtype {value.dtype} differs from cache dtype {dtype}")
+    if heads != Hkv:
+        raise ValueError(f"kv_cache holds {Hkv} KV heads, not {heads}")
     _require_cuda(slot_mapping, "slot_mapping")
-    if slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1 or slot_mapping.numel() != key.size(0):
+    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (T,):
         raise ValueError("slot_mapping must be int64 [T]")
-    _same_device(kv_cache.device, key=key, value=value, slot_mapping=slot_mapping)
+    slot_mapping = slot_mapping.contiguous()
+    index = kv_cache.get_device()
+    _on_device(index, key, "key")
+    _on_device(index, value, "value")
+    _on_device(index, slot_mapping, "slot_mapping")
+    _launch(index, what, fn, key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0), base, block_stride, N,
+            slot_mapping.data_ptr(), T, Hkv, D, _DTYPES[dtype])
 
 
 def reshape_and_cache_int4(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, layer: int,
@@ -581,15 +625,7 @@ def reshape_and_cache_int4(key: torch.Tensor, value: torch.Tensor, kv_cache: tor
     minimum`` with a 4-bit code; a group with a NaN or an infinity reads back as NaN. The slots of one
     call must be distinct.
     """
-    base = _int4_layer(kv_cache, layer, key.size(1) if isinstance(key, torch.Tensor) and key.dim() == 3 else None)
-    _int4_rows(key, value, kv_cache, slot_mapping)
-    slot_mapping = slot_mapping.contiguous()
-    dev = kv_cache.device
-    with torch.cuda.device(dev):
-        st = lib.aeg_reshape_and_cache_int4(key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0), base,
-                                            kv_cache.stride(0), kv_cache.size(0), slot_mapping.data_ptr(), key.size(0),
-                                            key.size(1), key.size(2), _DTYPES[kv_cache.dtype], _stream(dev))
-    check(st, "reshape_and_cache_int4")
+    _int4_move(lib.aeg_reshape_and_cache_int4, "reshape_and_cache_int4", key, value, kv_cache, layer, slot_mapping)
 
 
 def gather_cache_int4(kv_cache: torch.Tensor, layer: int, slot_mapping: torch.Tensor, key: torch.Tensor | None = None,
@@ -597,24 +633,17 @@ def gather_cache_int4(kv_cache: torch.Tensor, layer: int, slot_mapping: torch.Te
     """Keys and values ``[T, Hkv, 128]`` held at ``slot_mapping`` (int64 ``[T]``) of ``layer``, in the
     cache's dtype: what a prompt that continues a cached prefix attends to, or what a 16-bit cache
     takes over. Slots < 0 give zero rows. ``key``/``value`` receive the result when given."""
-    base = _int4_layer(kv_cache, layer)
     if (key is None) != (value is None):
         raise ValueError("key and value are given together")
     if key is None:
+        _require_cuda(kv_cache, "kv_cache")
         _require_cuda(slot_mapping, "slot_mapping")
+        if kv_cache.dim() != 4:
+            raise ValueError(f"kv_cache must be a 4-bit cache (N, L, Hkv, {INT4_TILE})")
         shape = (slot_mapping.numel(), kv_cache.size(2), 128)
         key = torch.empty(shape, dtype=kv_cache.dtype, device=kv_cache.device)
         value = torch.empty_like(key)
-    elif key.dim() != 3 or key.size(1) != kv_cache.size(2):
-        raise ValueError("key and value must be [T, Hkv, 128] with the cache's Hkv")
-    _int4_rows(key, value, kv_cache, slot_mapping)
-    slot_mapping = slot_mapping.contiguous()
-    dev = kv_cache.device
-    with torch.cuda.device(dev):
-        st = lib.aeg_gather_cache_int4(key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0), base,
-                                       kv_cache.stride(0), kv_cache.size(0), slot_mapping.data_ptr(), key.size(0),
-                                       key.size(1), key.size(2), _DTYPES[kv_cache.dtype], _stream(dev))
-    check(st, "gather_cache_int4")
+    _int4_move(lib.aeg_gather_cache_int4, "gather_cache_int4", key, value, kv_cache, layer, slot_mapping)
     return key, value
 
 
@@ -651,76 +680,92 @@ def rotary_multi_axis(query: torch.Tensor, key: torch.Tensor, positions: torch.T
     are dims (i, i + half); dims from ``2 * half`` on are copied. ``scaling`` multiplies the rotated
     dims. Returns new tensors unless ``query_out``/``key_out`` are given; those may be the inputs.
     """
-    for name, t in (("query", query), ("key", key)):
-        _require_cuda(t, name)
-        if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.size(2):
-            raise ValueError(f"{name} must be [T, heads, D] with contiguous heads")
-    if query.dtype not in _DTYPES or key.dtype != query.dtype:
+    T, Hq, D = q_shape = _token_rows(query, "query", "[T, Hq, D]")
+    k_shape = _token_rows(key, "key", "[T, Hkv, D]")
+    dtype = query.dtype
+    if dtype not in _DTYPES or key.dtype != dtype:
         raise ValueError("query and key must share an fp16 or bf16 dtype")
-    T, Hq, D = query.shape
-    if key.size(0) != T or key.size(2) != D:
+    if k_shape[0] != T or k_shape[2] != D:
         raise ValueError("query and key must have the same tokens and head_dim")
-    axis_of = _axis_of(tuple(sections), bool(interleaved))
-    half = len(axis_of)
+    sections = tuple(sections)
+    axis_of = _axis_of(sections, bool(interleaved))
+    half, axes = len(axis_of), len(sections)
     _require_cuda(positions, "positions")
     _require_cuda(inv_freq, "inv_freq")
     if positions.dim() == 1:
         positions = positions.unsqueeze(0)
-    if positions.dtype != torch.int64 or tuple(positions.shape) != (len(sections), T):
-        raise ValueError(f"positions must be int64 [{len(sections)}, {T}]")
-    if positions.stride(1) != 1 or positions.stride(0) < T:
+    if positions.dtype != torch.int64 or positions.shape != (axes, T):
+        raise ValueError(f"positions must be int64 [{axes}, {T}]")
+    axis_stride, step = positions.stride()
+    if (step != 1 and T > 1) or axis_stride < T:
         positions = positions.contiguous()
+        axis_stride = T
     if inv_freq.dtype != torch.float32 or inv_freq.shape != (half,):
         raise ValueError(f"inv_freq must be float32 [{half}], one per frequency of the sections")
     inv_freq = inv_freq.contiguous()
+    index = query.get_device()
+    for name, t in (("key", key), ("positions", positions), ("inv_freq", inv_freq)):
+        _on_device(index, t, name)
     if query_out is None:
-        query_out = torch.empty((T, Hq, D), dtype=query.dtype, device=query.device)
+        query_out = torch.empty(q_shape, dtype=dtype, device=query.device)
+    else:
+        _check_rotary_out(index, query_out, query, "query_out")
     if key_out is None:
-        key_out = torch.empty(key.shape, dtype=key.dtype, device=key.device)
-    for name, out, src in (("query_out", query_out, query), ("key_out", key_out, key)):
-        if out.shape != src.shape or out.dtype != src.dtype or out.stride(2) != 1 or out.stride(1) != D:
-            raise ValueError(f"{name} must match its input's shape and dtype, with contiguous heads")
-        if out.data_ptr() == src.data_ptr() and out.stride(0) != src.stride(0):
-            raise ValueError(f"{name} shares its input's memory with another stride")
-    dev = query.device
-    _same_device(dev, key=key, positions=positions, inv_freq=inv_freq, query_out=query_out, key_out=key_out)
-    with torch.cuda.device(dev):
-        st = lib.aeg_rotary_multi_axis(query_out.data_ptr(), query_out.stride(0), key_out.data_ptr(), key_out.stride(0),
-                                       query.data_ptr(), query.stride(0), key.data_ptr(), key.stride(0),
-                                       positions.data_ptr(), positions.stride(0), len(sections), inv_freq.data_ptr(),
-                                       axis_of, half, float(scaling), T, Hq, key.size(1), D, _DTYPES[query.dtype],
-                                       _stream(dev))
-    check(st, "rotary_multi_axis")
+        key_out = torch.empty(k_shape, dtype=dtype, device=key.device)
+    else:
+        _check_rotary_out(index, key_out, key, "key_out")
+    _launch(index, "rotary_multi_axis", lib.aeg_rotary_multi_axis, query_out.data_ptr(), query_out.stride(0),
+            key_out.data_ptr(), key_out.stride(0), query.data_ptr(), query.stride(0), key.data_ptr(), key.stride(0),
+            positions.data_ptr(), axis_stride, axes, inv_freq.data_ptr(), axis_of, half, float(scaling), T, Hq, k_shape[1], D,
+            _DTYPES[dtype])
     return query_out, key_out
+
+
+def _check_rotary_out(index: int, out: torch.Tensor, src: torch.Tensor, name: str) -> None:
+    shape = _token_rows(out, name, "its input's shape")
+    if shape != src.shape or out.dtype != src.dtype:
+        raise ValueError(f"{name} must match its input's shape and dtype")
+    if out.data_ptr() == src.data_ptr() and out.stride(0) != src.stride(0):
+        raise ValueError(f"{name} shares its input's memory with another stride")
+    _on_device(index, out, name)
 
 
 # --------------------------------------------------------------------------------------------
 # Shared blocks: forking, freeing and compacting over reference counts
 
 
-def _check_shared(ref_counts: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor) -> torch.device:
-    for t, name in ((ref_counts, "ref_counts"), (block_tables, "block_tables"), (seq_lens, "seq_lens")):
+def _check_shared(ref_counts: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor):
+    """Checks the state; returns (device index, blocks, table width, rows)."""
+    for t, name, dims in ((ref_counts, "ref_counts", 1), (block_tables, "block_tables", 2), (seq_lens, "seq_lens", 1)):
         _require_cuda(t, name)
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 tensor")
-    if ref_counts.dim() != 1 or block_tables.dim() != 2 or seq_lens.dim() != 1:
-        raise ValueError("ref_counts must be [num_blocks], block_tables [rows, W] and seq_lens [rows]")
-    if seq_lens.numel() != block_tables.size(0):
+        if t.dtype != torch.int32 or t.dim() != dims or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor, ref_counts [num_blocks], block_tables [rows, W], "
+                             "seq_lens [rows]")
+    rows, width = block_tables.shape
+    if seq_lens.size(0) != rows:
         raise ValueError("seq_lens must have one entry per table row")
-    if block_tables.size(1) == 0:
+    if width == 0:
         raise ValueError("block_tables has no columns")
-    dev = ref_counts.device
-    _same_device(dev, block_tables=block_tables, seq_lens=seq_lens)
-    return dev
+    index = ref_counts.get_device()
+    _on_device(index, block_tables, "block_tables")
+    _on_device(index, seq_lens, "seq_lens")
+    return index, ref_counts.size(0), width, rows
 
 
-def _check_pool(kv_cache: torch.Tensor, ref_counts: torch.Tensor) -> None:
-    _require_cuda(kv_cache, "kv_cache")
-    if not kv_cache.is_contiguous() or kv_cache.dim() < 1:
+def _check_pool(kv_cache: torch.Tensor, index: int, num_blocks: int) -> int:
+    """Checks a block pool; returns the bytes of a block."""
+    _on_device(index, kv_cache, "kv_cache")
+    if kv_cache.dim() < 1 or not kv_cache.is_contiguous():
         raise ValueError("kv_cache must be contiguous")
-    if kv_cache.size(0) != ref_counts.numel():
-        raise ValueError(f"kv_cache has {kv_cache.size(0)} blocks but ref_counts {ref_counts.numel()} entries")
-    _same_device(ref_counts.device, kv_cache=kv_cache)
+    if kv_cache.size(0) != num_blocks:
+        raise ValueError(f"kv_cache has {kv_cache.size(0)} blocks but ref_counts {num_blocks} entries")
+    return block_bytes(kv_cache)
+
+
+def _row_ids(rows, ref_counts: torch.Tensor, index: int, name: str) -> torch.Tensor:
+    if isinstance(rows, torch.Tensor) and rows.dtype == torch.int64 and rows.get_device() == index and rows.dim() == 1:
+        return rows.contiguous()
+    return _device_ids(rows, ref_counts.device, name)
 
 
 def fork_blocks(kv_cache: torch.Tensor, ref_counts: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
@@ -737,38 +782,35 @@ def fork_blocks(kv_cache: torch.Tensor, ref_counts: torch.Tensor, block_tables: 
     (``read_device_errors``): a row out of range, a target row that is not empty or named before, a
     pool with no free block left.
     """
-    dev = _check_shared(ref_counts, block_tables, seq_lens)
-    _check_pool(kv_cache, ref_counts)
-    src = _device_ids(src_rows, dev, "src_rows")
-    dst = _device_ids(dst_rows, dev, "dst_rows")
-    n = src.numel()
-    if dst.numel() != n:
-        raise ValueError(f"{n} source rows but {dst.numel()} target rows")
-    new_blocks = torch.empty(n, dtype=torch.int32, device=dev)
+    index, N, width, rows = _check_shared(ref_counts, block_tables, seq_lens)
+    nbytes = _check_pool(kv_cache, index, N)
+    src = _row_ids(src_rows, ref_counts, index, "src_rows")
+    dst = _row_ids(dst_rows, ref_counts, index, "dst_rows")
+    n = src.size(0)
+    if dst.size(0) != n:
+        raise ValueError(f"{n} source rows but {dst.size(0)} target rows")
+    # One allocation: the result, then the entries' scratch (16-byte aligned).
+    ws_bytes = lib.aeg_fork_blocks_workspace_size(n)
+    at = (n + 3) // 4 * 4
+    buf = torch.empty(at + (ws_bytes + 3) // 4, dtype=torch.int32, device=ref_counts.device)
+    new_blocks = buf[:n]
     if n == 0:
         return new_blocks
-    ws = torch.empty(lib.aeg_fork_blocks_workspace_size(n), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        st = lib.aeg_fork_blocks(kv_cache.data_ptr(), block_bytes(kv_cache), ref_counts.numel(), ref_counts.data_ptr(),
-                                 block_tables.data_ptr(), block_tables.size(1), block_tables.size(0),
-                                 seq_lens.data_ptr(), src.data_ptr(), dst.data_ptr(), n, new_blocks.data_ptr(),
-                                 ws.data_ptr(), ws.numel(), _stream(dev))
-    check(st, "fork_blocks")
+    ptr = buf.data_ptr()
+    _launch(index, "fork_blocks", lib.aeg_fork_blocks, kv_cache.data_ptr(), nbytes, N, ref_counts.data_ptr(),
+            block_tables.data_ptr(), width, rows, seq_lens.data_ptr(), src.data_ptr(), dst.data_ptr(), n, ptr, ptr + 4 * at,
+            ws_bytes)
     return new_blocks
 
 
 def free_blocks(ref_counts: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, rows) -> None:
     """Empties the table rows ``rows``: every block of a row gives back one reference (a block at 0 is
     free), and the row's length becomes 0. A row named twice is freed once."""
-    dev = _check_shared(ref_counts, block_tables, seq_lens)
-    ids = _device_ids(rows, dev, "rows")
-    if ids.numel() == 0:
-        return
-    with torch.cuda.device(dev):
-        st = lib.aeg_free_blocks(ref_counts.numel(), ref_counts.data_ptr(), block_tables.data_ptr(),
-                                 block_tables.size(1), block_tables.size(0), seq_lens.data_ptr(), ids.data_ptr(),
-                                 ids.numel(), _stream(dev))
-    check(st, "free_blocks")
+    index, N, width, n_rows = _check_shared(ref_counts, block_tables, seq_lens)
+    ids = _row_ids(rows, ref_counts, index, "rows")
+    if ids.size(0):
+        _launch(index, "free_blocks", lib.aeg_free_blocks, N, ref_counts.data_ptr(), block_tables.data_ptr(), width, n_rows,
+                seq_lens.data_ptr(), ids.data_ptr(), ids.size(0))
 
 
 class CompactedBlocks(NamedTuple):
@@ -789,19 +831,14 @@ def compact_blocks(kv_cache: torch.Tensor, ref_counts: torch.Tensor, block_table
     ``seq_lens`` are only read: adopt the returned tables and counts. The old places keep their
     contents, so a step in flight on the old tables stays right until their ids are given out.
     """
-    dev = _check_shared(ref_counts, block_tables, seq_lens)
-    _check_pool(kv_cache, ref_counts)
-    N = ref_counts.numel()
+    index, N, width, rows = _check_shared(ref_counts, block_tables, seq_lens)
+    nbytes = _check_pool(kv_cache, index, N)
     out = CompactedBlocks(torch.empty_like(block_tables), torch.empty_like(ref_counts), torch.empty_like(ref_counts),
-                          torch.empty(1, dtype=torch.int32, device=dev))
-    ws = torch.empty(lib.aeg_compact_blocks_workspace_size(N), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        st = lib.aeg_compact_blocks(kv_cache.data_ptr(), block_bytes(kv_cache), N, ref_counts.data_ptr(),
-                                    block_tables.data_ptr(), block_tables.size(1), block_tables.size(0),
-                                    seq_lens.data_ptr(), out.ref_counts.data_ptr(), out.block_tables.data_ptr(),
-                                    out.remap.data_ptr(), out.num_live.data_ptr(), ws.data_ptr(), ws.numel(),
-                                    _stream(dev))
-    check(st, "compact_blocks")
+                          torch.empty(1, dtype=torch.int32, device=ref_counts.device))
+    ws = torch.empty(lib.aeg_compact_blocks_workspace_size(N), dtype=torch.uint8, device=ref_counts.device)
+    _launch(index, "compact_blocks", lib.aeg_compact_blocks, kv_cache.data_ptr(), nbytes, N, ref_counts.data_ptr(),
+            block_tables.data_ptr(), width, rows, seq_lens.data_ptr(), out.ref_counts.data_ptr(),
+            out.block_tables.data_ptr(), out.remap.data_ptr(), out.num_live.data_ptr(), ws.data_ptr(), ws.size(0))
     return out
 
 
@@ -842,22 +879,22 @@ class DecodePlan:
         [B, W]) on the current stream. Both must stay unchanged while the plan is in use."""
         _require_cuda(seq_lens, "seq_lens")
         _require_cuda(block_tables, "block_tables")
-        if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or seq_lens.numel() != self.batch:
+        if seq_lens.dtype != torch.int32 or seq_lens.shape != (self.batch,):
             raise ValueError(f"seq_lens must be int32 [{self.batch}]")
         if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.size(0) != self.batch:
             raise ValueError(f"block_tables must be int32 [{self.batch}, W]")
         if block_tables.size(1) == 0:
             raise ValueError("block_tables has no columns")
-        _same_device(self.device, seq_lens=seq_lens, block_tables=block_tables)
+        index = self.device.index
+        _on_device(index, seq_lens, "seq_lens")
+        _on_device(index, block_tables, "block_tables")
         seq_lens = seq_lens.contiguous()
         if block_tables.stride(1) != 1:
             block_tables = block_tables.contiguous()
-        plan = lib.aeg_decode_plan_int4 if self.cache == "int4" else lib.aeg_decode_plan
-        with torch.cuda.device(self.device):
-            st = plan(self.workspace.data_ptr(), self.workspace.numel(), block_tables.data_ptr(), block_tables.stride(0),
-                      seq_lens.data_ptr(), self.batch, self.num_q_heads, self.num_kv_heads, self.head_dim,
-                      _stream(self.device))
-        check(st, "decode_plan")
+        int4 = self.cache == "int4"
+        _launch(index, "decode_plan_int4" if int4 else "decode_plan", lib.aeg_decode_plan_int4 if int4 else lib.aeg_decode_plan,
+                self.workspace.data_ptr(), self.workspace.numel(), block_tables.data_ptr(), block_tables.stride(0),
+                seq_lens.data_ptr(), self.batch, self.num_q_heads, self.num_kv_heads, self.head_dim)
         self.table_width = block_tables.size(1)
         self.seq_lens = seq_lens
         self.block_tables = block_tables
@@ -1041,14 +1078,11 @@ def paged_attention_decode_int4(out: torch.Tensor, query: torch.Tensor, kv_cache
     this stream writes neither this layer's blocks nor the block tables (so not right after the
     layer's ``reshape_and_cache_int4``).
     """
-    _require_cuda(query, "query")
-    if query.dim() != 3 or query.stride(2) != 1 or query.stride(1) != query.size(2):
-        raise ValueError("query must be [B, Hq, D] with contiguous heads")
-    B, Hq, D = query.shape
-    base = _int4_layer(kv_cache, layer)
-    Hkv = kv_cache.size(2)
-    if query.dtype != kv_cache.dtype:
-        raise ValueError(f"query dtype {query.dtype} differs from cache dtype {kv_cache.dtype}")
+    B, Hq, D = shape = _token_rows(query, "query", "[B, Hq, D]")
+    base, block_stride, N, Hkv = _int4_layer(kv_cache, layer)
+    dtype = query.dtype
+    if dtype != kv_cache.dtype:
+        raise ValueError(f"query dtype {dtype} differs from cache dtype {kv_cache.dtype}")
     _require_cuda(block_tables, "block_tables")
     _require_cuda(seq_lens, "seq_lens")
     if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.size(0) != B:
@@ -1058,9 +1092,13 @@ def paged_attention_decode_int4(out: torch.Tensor, query: torch.Tensor, kv_cache
     if seq_lens.dtype != torch.int32 or seq_lens.shape != (B,):
         raise ValueError("seq_lens must be int32 [B]")
     seq_lens = seq_lens.contiguous()
-    _require_cuda(out, "out")
-    if out.shape != query.shape or out.dtype != query.dtype or out.stride(2) != 1 or out.stride(1) != D:
-        raise ValueError("out must match query's shape/dtype with contiguous heads")
+    if _token_rows(out, "out", "query's shape") != shape or out.dtype != dtype:
+        raise ValueError("out must match query's shape and dtype")
+    index = query.get_device()
+    _on_device(index, kv_cache, "kv_cache")
+    _on_device(index, block_tables, "block_tables")
+    _on_device(index, seq_lens, "seq_lens")
+    _on_device(index, out, "out")
     if B == 0:
         return
     if block_tables.size(1) == 0:
@@ -1069,13 +1107,9 @@ def paged_attention_decode_int4(out: torch.Tensor, query: torch.Tensor, kv_cache
         plan = DecodePlan(B, Hq, Hkv, D, query.device, cache="int4").plan(seq_lens, block_tables)
     elif not plan.matches(B, Hq, Hkv, D, block_tables, seq_lens, "int4"):
         raise ValueError("plan was built for a different batch / head layout / block tables / sequence lengths / cache")
-    dev = query.device
-    _same_device(dev, kv_cache=kv_cache, block_tables=block_tables, seq_lens=seq_lens, out=out,
-                 plan_workspace=plan.workspace)
-    with torch.cuda.device(dev):
-        st = lib.aeg_paged_attn_decode_int4(out.data_ptr(), out.stride(0), query.data_ptr(), query.stride(0), base,
-                                            kv_cache.stride(0), kv_cache.size(0), block_tables.data_ptr(),
-                                            block_tables.stride(0), seq_lens.data_ptr(), B, Hq, Hkv, D, float(scale),
-                                            _DTYPES[query.dtype], plan.workspace.data_ptr(), plan.workspace.numel(),
-                                            AEG_DECODE_PREFETCH if prefetch else 0, _stream(dev))
-    check(st, "paged_attention_decode_int4")
+    ws = plan.workspace
+    _on_device(index, ws, "plan workspace")
+    _launch(index, "paged_attention_decode_int4", lib.aeg_paged_attn_decode_int4, out.data_ptr(), out.stride(0),
+            query.data_ptr(), query.stride(0), base, block_stride, N, block_tables.data_ptr(), block_tables.stride(0),
+            seq_lens.data_ptr(), B, Hq, Hkv, D, float(scale), _DTYPES[dtype], ws.data_ptr(), ws.numel(),
+            AEG_DECODE_PREFETCH if prefetch else 0)
