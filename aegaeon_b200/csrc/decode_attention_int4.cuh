@@ -576,10 +576,8 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
     };
 
     // Adds the tile in stage `st` with scores x. Tokens from `valid` on get no weight and, whatever their
-    // value pairs hold, count as zeros. With kNext the next tile's scores are made on the way: their
-    // chain of MMAs runs beside this tile's exponents and products.
-    auto add_tile = [&](auto next_tag, uint32_t st, uint32_t st_next, float (*x)[4], float (*x_next)[4]) {
-      constexpr bool kNext = decltype(next_tag)::value;
+    // value pairs hold, count as zeros.
+    auto add_tile = [&](uint32_t st, float (*x)[4]) {
       const uint8_t* tile = ring + st * kInt4TileBytes;
       const int valid = wk.tokens[st];
       uint2 vp0 = lds64(tile + kInt4ValuePairs + grp * 8), vp1 = lds64(tile + kInt4ValuePairs + 64 + grp * 8);
@@ -602,7 +600,6 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
         for (int i = 0; i < 2; ++i) over = over || fmaxf(x[nt][i], x[nt][i + 2]) > mt_[nt][i];
       if (__any_sync(0xffffffffu, over)) make_room(x, vtop);
 
-      if constexpr (kNext) scores(st_next, x_next);
       const uint8_t* vcodes = tile + kInt4ValueCodes + quad * 128 + grp * 16;
       const uint4 vc0 = lds128(vcodes), vc1 = lds128(vcodes + 512);
 
@@ -646,30 +643,20 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
       }
     };
 
-    float x[NT][4], x_next[NT][4];
-    wait(&wk.full[st_con], ph_con);
-    if (lost) break;
-    scores(st_con, x);
+    float x[NT][4];
     for (int k = 0; k < n; ++k) {
-      const bool wraps = st_con + 1 == kSt;
-      const uint32_t st_next = wraps ? 0 : st_con + 1, ph_next = wraps ? ph_con ^ 1 : ph_con;
-      if (k + 1 < n) {
-        wait(&wk.full[st_next], ph_next);
-        if (lost) break;
-        add_tile(std::true_type{}, st_con, st_next, x, x_next);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[nt][i] = x_next[nt][i];
-      } else {
-        add_tile(std::false_type{}, st_con, st_next, x, x_next);
-      }
+      wait(&wk.full[st_con], ph_con);
+      if (lost) break;
+      scores(st_con, x);
+      add_tile(st_con, x);
       if ((k & (kFold - 1)) == kFold - 1) fold();
       // Every lane's reads of the stage have fed its products.
       __syncwarp();
       if (lane == 0) mbar_arrive(&wk.empty[st_con]);
-      st_con = st_next;
-      ph_con = ph_next;
+      if (++st_con == kSt) {
+        st_con = 0;
+        ph_con ^= 1;
+      }
     }
     if (lost) break;
 
