@@ -5,8 +5,9 @@
 // Both are bound by memory: 512 bytes of keys and values a (token, head) on one side, 144 bytes of
 // codes and pairs on the other. One warp moves one (token, head): lanes 0..15 its key, 16..31 its
 // value, 8 dims a lane (one 16-byte vector), 8 lanes a 64-dim group, so that a group's range is
-// three shuffles away and a lane's codes are exactly one key word or two value halves. A warp takes
-// kItems of them at a time, all loads before the first use.
+// three shuffles away and a lane's codes are exactly one key word or two value halves. Where there are
+// enough of them a warp takes kTokens tokens x kHeads heads at a time, all loads before the first use; the
+// heads' chunks are the grid's second dimension, so that no index is divided.
 #include "int4_tile.cuh"
 
 #include <algorithm>
@@ -53,32 +54,32 @@ struct Rows {
   int64_t block_stride;  // bytes between blocks
   const int64_t* slots;
   int64_t num_slots;
-  int64_t items;  // tokens * heads
+  int64_t tokens;
   int heads;
 };
 
-template <typename T, bool kVec, int kItems>
+template <typename T, bool kVec, int kTokens, int kHeads>
 __global__ void __launch_bounds__(kThreads) write_int4_kernel(const Rows p) {
+  constexpr int kItems = kTokens * kHeads;
   pdl_launch_dependents();
   pdl_wait_primary();
   const int lane = threadIdx.x & 31, l = lane & 15;
   const bool is_key = lane < 16;
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarpsPerCta;
-  const int64_t warp = static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5);
-  const uint16_t* rows = is_key ? p.key : p.value;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarpsPerCta * kTokens;
+  const int h0 = blockIdx.y * kHeads;
   const int64_t stride = is_key ? p.key_stride : p.value_stride;
-  for (int64_t i0 = warp * kItems; i0 < p.items; i0 += warps * kItems) {
+  const uint16_t* rows = (is_key ? p.key : p.value) + h0 * kInt4Dim + 8 * l;
+  uint8_t* tiles = p.cache + static_cast<int64_t>(h0) * kInt4TileBytes;
+  const int pairs_at = (is_key ? kInt4KeyPairs : kInt4ValuePairs) + (l >> 3) * 4;
+  for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5)) * kTokens; t0 < p.tokens; t0 += step) {
     uint4 v[kItems];
-    int64_t slot[kItems];
-    int head[kItems];
+    int64_t slot[kTokens];
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
-      const int64_t i = min(i0 + k, p.items - 1);
-      const int64_t t = i / p.heads;
-      head[k] = static_cast<int>(i - t * p.heads);
-      slot[k] = p.slots[t];
-      v[k] = load8<kVec>(rows + t * stride + head[k] * kInt4Dim + 8 * l);
-      if (i0 + k >= p.items) slot[k] = -1;
+      const int64_t t = t0 + k / kHeads;
+      const bool there = t < p.tokens && h0 + k % kHeads < p.heads;
+      if (k % kHeads == 0) slot[k / kHeads] = t < p.tokens ? p.slots[t] : -1;
+      v[k] = there ? load8<kVec>(rows + t * stride + (k % kHeads) * kInt4Dim) : make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
@@ -90,74 +91,74 @@ __global__ void __launch_bounds__(kThreads) write_int4_kernel(const Rows p) {
         x[2 * n] = f.x;
         x[2 * n + 1] = f.y;
       }
-      uint32_t word, pair;
-      int4_quantise<T>(x, word, pair);
-      if (slot[k] >= p.num_slots) {
+      const uint2 q = int4_quantise<T>(x);
+      const int64_t s = slot[k / kHeads];
+      if (s >= p.num_slots) {
         if (lane == 0) atomicOr(&g_deverr_int4, AEG_DEVERR_SLOT_RANGE);
-      } else if (slot[k] >= 0) {
-        const int t = static_cast<int>(slot[k] & 15);
-        uint8_t* tile = p.cache + (slot[k] >> 4) * p.block_stride + static_cast<int64_t>(head[k]) * kInt4TileBytes;
+      } else if (s >= 0 && h0 + k % kHeads < p.heads) {
+        const int t = static_cast<int>(s & 15);
+        uint8_t* tile = tiles + (s >> 4) * p.block_stride + (k % kHeads) * kInt4TileBytes;
         if (is_key) {
-          *reinterpret_cast<uint32_t*>(tile + int4_key_word(t, l)) = word;
+          *reinterpret_cast<uint32_t*>(tile + int4_key_word(t, l)) = q.x;
         } else {
           uint16_t* half = reinterpret_cast<uint16_t*>(tile + int4_value_half(t, l));
-          half[0] = static_cast<uint16_t>(word);
-          half[2] = static_cast<uint16_t>(word >> 16);
+          half[0] = static_cast<uint16_t>(q.x);
+          half[2] = static_cast<uint16_t>(q.x >> 16);
         }
-        if ((l & 7) == 0)
-          *reinterpret_cast<uint32_t*>(tile + (is_key ? kInt4KeyPairs : kInt4ValuePairs) + t * 8 + (l >> 3) * 4) = pair;
+        if ((l & 7) == 0) *reinterpret_cast<uint32_t*>(tile + pairs_at + t * 8) = q.y;
       }
     }
   }
 }
 
-template <typename T, bool kVec, int kItems>
+template <typename T, bool kVec, int kTokens, int kHeads>
 __global__ void __launch_bounds__(kThreads) gather_int4_kernel(const Rows p) {
+  constexpr int kItems = kTokens * kHeads;
   pdl_launch_dependents();
   pdl_wait_primary();
   const int lane = threadIdx.x & 31, l = lane & 15;
   const bool is_key = lane < 16;
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarpsPerCta;
-  const int64_t warp = static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5);
-  uint16_t* rows = is_key ? p.key : p.value;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarpsPerCta * kTokens;
+  const int h0 = blockIdx.y * kHeads;
   const int64_t stride = is_key ? p.key_stride : p.value_stride;
-  for (int64_t i0 = warp * kItems; i0 < p.items; i0 += warps * kItems) {
+  uint16_t* rows = (is_key ? p.key : p.value) + h0 * kInt4Dim + 8 * l;
+  const uint8_t* tiles = p.cache + static_cast<int64_t>(h0) * kInt4TileBytes;
+  const int pairs_at = (is_key ? kInt4KeyPairs : kInt4ValuePairs) + (l >> 3) * 4;
+  for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5)) * kTokens; t0 < p.tokens; t0 += step) {
     uint32_t word[kItems], pair[kItems];
-    int64_t token[kItems], slot[kItems];
+    int64_t slot[kTokens];
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      token[k] = min(i0 + k, p.items - 1) / p.heads;
-      slot[k] = p.slots[token[k]];
+    for (int j = 0; j < kTokens; ++j) {
+      slot[j] = t0 + j < p.tokens ? p.slots[t0 + j] : -1;
+      if (slot[j] >= p.num_slots && lane == 0) atomicOr(&g_deverr_int4, AEG_DEVERR_SLOT_RANGE);
     }
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
       word[k] = 0;
       pair[k] = 0;  // scale 0, minimum 0: zeros
-      if (slot[k] >= 0 && slot[k] < p.num_slots) {
-        const int head = static_cast<int>(min(i0 + k, p.items - 1) - token[k] * p.heads);
-        const int t = static_cast<int>(slot[k] & 15);
-        const uint8_t* tile = p.cache + (slot[k] >> 4) * p.block_stride + static_cast<int64_t>(head) * kInt4TileBytes;
+      const int64_t s = slot[k / kHeads];
+      if (s >= 0 && s < p.num_slots && h0 + k % kHeads < p.heads) {
+        const int t = static_cast<int>(s & 15);
+        const uint8_t* tile = tiles + (s >> 4) * p.block_stride + (k % kHeads) * kInt4TileBytes;
         if (is_key) {
           word[k] = *reinterpret_cast<const uint32_t*>(tile + int4_key_word(t, l));
         } else {
           const uint16_t* half = reinterpret_cast<const uint16_t*>(tile + int4_value_half(t, l));
           word[k] = half[0] | (uint32_t(half[2]) << 16);
         }
-        pair[k] = *reinterpret_cast<const uint32_t*>(tile + (is_key ? kInt4KeyPairs : kInt4ValuePairs) + t * 8 + (l >> 3) * 4);
-      } else if (slot[k] >= p.num_slots && lane == 0) {
-        atomicOr(&g_deverr_int4, AEG_DEVERR_SLOT_RANGE);
+        pair[k] = *reinterpret_cast<const uint32_t*>(tile + pairs_at + t * 8);
       }
     }
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
-      if (i0 + k >= p.items) break;
+      const int64_t t = t0 + k / kHeads;
+      if (t >= p.tokens || h0 + k % kHeads >= p.heads) continue;
       const float2 sm = unpack2<T>(pair[k]);
       // One rounding to fp32 (code * scale alone is exact), one to the type.
       auto value = [&](int n) { return fmaf(static_cast<float>((word[k] >> (4 * n)) & 15u), sm.x, sm.y); };
-      const uint4 out = make_uint4(pack2<T>(value(0), value(1)), pack2<T>(value(2), value(3)),
-                                   pack2<T>(value(4), value(5)), pack2<T>(value(6), value(7)));
-      const int64_t head = i0 + k - token[k] * p.heads;
-      store8<kVec>(rows + token[k] * stride + head * kInt4Dim + 8 * l, out);
+      store8<kVec>(rows + t * stride + (k % kHeads) * kInt4Dim,
+                   make_uint4(pack2<T>(value(0), value(1)), pack2<T>(value(2), value(3)), pack2<T>(value(4), value(5)),
+                              pack2<T>(value(6), value(7))));
     }
   }
 }
@@ -187,35 +188,45 @@ int prepare(const char* what, Rows& p, const void* key, const void* value, int64
   p.block_stride = 2 * block_stride;
   p.slots = slot_mapping;
   p.num_slots = num_blocks * 16;
-  p.items = T * Hkv;
+  p.tokens = T;
   p.heads = Hkv;
   return AEG_OK;
 }
 
 using Kernel = void (*)(const Rows);
 
-template <typename T, int kItems>
+template <typename T, int kTokens, int kHeads>
 Kernel pick(bool write, bool vec) {
-  if (write) return vec ? write_int4_kernel<T, true, kItems> : write_int4_kernel<T, false, kItems>;
-  return vec ? gather_int4_kernel<T, true, kItems> : gather_int4_kernel<T, false, kItems>;
+  if (write) return vec ? write_int4_kernel<T, true, kTokens, kHeads> : write_int4_kernel<T, false, kTokens, kHeads>;
+  return vec ? gather_int4_kernel<T, true, kTokens, kHeads> : gather_int4_kernel<T, false, kTokens, kHeads>;
 }
 
-constexpr int kManyItems = 4;
+// Several (token, head) a warp only where every resident warp has as many; then 4, of one token where it
+// has 4 heads.
+template <typename T>
+Kernel pick(bool write, bool vec, int64_t items, int heads, int* tokens, int* chunk) {
+  const bool many = items >= int64_t(num_sms()) * 16 * kWarpsPerCta;
+  *chunk = !many || heads == 1 ? 1 : (heads < 4 ? 2 : 4);
+  *tokens = many ? 4 / *chunk : 1;
+  if (!many) return pick<T, 1, 1>(write, vec);
+  return heads == 1 ? pick<T, 4, 1>(write, vec) : (heads < 4 ? pick<T, 2, 2>(write, vec) : pick<T, 1, 4>(write, vec));
+}
 
 int launch(const char* what, bool write, const Rows& p, int dtype, cudaStream_t stream) {
   const bool vec = aligned(p.key, 16) && aligned(p.value, 16) && p.key_stride % 8 == 0 && p.value_stride % 8 == 0;
-  // Several items a warp only once every SM's warps have one.
-  const int64_t resident = int64_t(num_sms()) * 16 * kWarpsPerCta;
-  const bool many = p.items >= resident;
-  const Kernel k = dtype == AEG_DTYPE_BF16
-                       ? (many ? pick<__nv_bfloat16, kManyItems>(write, vec) : pick<__nv_bfloat16, 1>(write, vec))
-                       : (many ? pick<__half, kManyItems>(write, vec) : pick<__half, 1>(write, vec));
-  const int64_t per_cta = int64_t(kWarpsPerCta) * (many ? kManyItems : 1);
+  int tokens = 1, chunk = 1;
+  const Kernel k = dtype == AEG_DTYPE_BF16 ? pick<__nv_bfloat16>(write, vec, p.tokens * p.heads, p.heads, &tokens, &chunk)
+                                           : pick<__half>(write, vec, p.tokens * p.heads, p.heads, &tokens, &chunk);
+  const int chunks = (p.heads + chunk - 1) / chunk;
+  AEG_CHECK_ARG(chunks <= 65535, "%s: %d KV heads are too many", what, p.heads);
+  const int64_t per_cta = int64_t(kWarpsPerCta) * tokens;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>((p.items + per_cta - 1) / per_cta, int64_t(num_sms()) * 16)));
+  const int64_t resident = std::max<int64_t>(int64_t(num_sms()) * 16 / chunks, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>((p.tokens + per_cta - 1) / per_cta, resident)),
+                     static_cast<unsigned>(chunks));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cfg.attrs = attr;

@@ -23,6 +23,8 @@
 
 #include "aeg_common.cuh"
 
+#include <type_traits>
+
 namespace aeg {
 
 constexpr int kInt4Dim = 128;
@@ -74,32 +76,29 @@ __device__ __forceinline__ float to_float<__half>(__half v) { return __half2floa
 template <>
 __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// Codes of a lane's 8 dims and its group's pair. The 8 lanes of a group are consecutive and call
-// this together. `word` holds dim n's code at bits 4 n; the pair is scale | minimum << 16.
-//
-// Codes are decided in fp32 without a rounding error in the decision: c = rint(d / s) by a
-// reciprocal is right or next to it, c * s has at most 15 bits, and d - c * s comes out of one FMA
-// exactly, as |d - c s| <= s and d <= 16 s or so. Only where it is exactly half a scale does the
-// rounding error e of d = x - minimum itself count.
+// A scale rounded as if from infinite precision, for an exact span: the quotient cut off at 24 bits with
+// a sticky last bit, then T's rounding.
 template <typename T>
-__device__ __forceinline__ void int4_quantise(const float (&x)[8], uint32_t& word, uint32_t& pair) {
-  float lo = x[0], hi = x[0];
-#pragma unroll
-  for (int n = 1; n < 8; ++n) {
-    lo = min_nan(lo, x[n]);
-    hi = max_nan(hi, x[n]);
-  }
-#pragma unroll
-  for (int off = 1; off < 8; off <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-  }
+__device__ __forceinline__ T scale_of_exact(float span) {
+  const float q = __fdiv_rz(span, 15.f);
+  const uint32_t sticky = fmaf(-15.f, q, span) != 0.f ? 1u : 0u;
+  return from_float<T>(__uint_as_float(__float_as_uint(q) | sticky));
+}
+
+__device__ __forceinline__ uint32_t pair_of(uint32_t scale, uint32_t lo) { return scale | (lo << 16); }
+
+// The general form of int4_quantise, right for every group. Codes: c = rint(d / s) by a reciprocal is
+// right or next to it, c * s has at most 15 bits, and d - c * s comes out of one FMA exactly, as
+// |d - c s| <= s and d <= 16 s or so. Only where it is exactly half a scale does the rounding error e of
+// d = x - minimum itself count.
+template <typename T>
+__device__ __noinline__ uint2 int4_quantise_any(const float (&x)[8], float lo, float hi) {
   const bool ok = isfinite(hi - lo);
   const T scale = round_once<T>(ok ? (static_cast<double>(hi) - static_cast<double>(lo)) / 15.0 : 0.0);
   float s = to_float<T>(scale);
-  word = 0;
-  pair = ok ? (bits16(scale) | (bits16(from_float<T>(lo)) << 16)) : 0x7fff7fffu;
-  if (!ok || s == 0.f) return;
+  uint32_t word = 0;
+  const uint32_t pair = ok ? pair_of(bits16(scale), bits16(from_float<T>(lo))) : 0x7fff7fffu;
+  if (!ok || s == 0.f) return make_uint2(0u, pair);
   // Far below 1, both sides are scaled up exactly so that the reciprocal stays finite.
   const float up = s < 1e-30f ? 18446744073709551616.f : 1.f;
   s *= up;
@@ -118,6 +117,51 @@ __device__ __forceinline__ void int4_quantise(const float (&x)[8], uint32_t& wor
     }
     word |= static_cast<uint32_t>(static_cast<int>(c)) << (4 * n);
   }
+  return make_uint2(word, pair);
+}
+
+// Codes of a lane's 8 dims and its group's pair: {codes, dim n's at bits 4 n; scale | minimum << 16}. The
+// 8 lanes of a group are consecutive; the whole warp calls this together.
+//
+// Where no element but 0 is below 2^(p - 23) of the span (p: T's significant bits), every x - minimum is
+// a multiple of 2^-23 of the span or more. Then differences are exact in fp32, a quotient that is no tie
+// differs from one by more than fp32's rounding, and a correctly rounded quotient gives the right code:
+// that is a product and two FMAs (Markstein's division with the rounded reciprocal), and adding 1.5 * 2^23
+// rounds it to a whole number, ties to even, with the code in the low bits. fp16 has no bits below 2^-24,
+// so any group with a span below 1/2 is fine too. Groups that are not sure of it, with subnormal scales
+// or without a finite span take the general form, with their warp. Writing a prompt batch of 11,348
+// tokens x 4 heads took 21.7 us with the general form alone.
+template <typename T>
+__device__ __forceinline__ uint2 int4_quantise(const float (&x)[8]) {
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  constexpr float kLeast = kHalf ? 0x1p-12f : 0x1p-15f;
+  constexpr float kNormal = kHalf ? 0x1p-14f : 1e-30f;  // least scale of the short form
+  float lo = x[0], hi = x[0], least = fabsf(x[0]);
+#pragma unroll
+  for (int n = 1; n < 8; ++n) {
+    lo = min_nan(lo, x[n]);
+    hi = max_nan(hi, x[n]);
+    least = fminf(least, fabsf(x[n]));
+  }
+#pragma unroll
+  for (int off = 1; off < 8; off <<= 1) {
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+    least = fminf(least, __shfl_xor_sync(0xffffffffu, least, off));
+  }
+  const float span = hi - lo;
+  const bool sure = (least > span * kLeast || (kHalf && span < 0.5f)) && span > 16.f * kNormal && span < 3e38f;
+  if (!__all_sync(0xffffffffu, sure)) return int4_quantise_any<T>(x, lo, hi);
+  const T scale = scale_of_exact<T>(span);
+  const float s = to_float<T>(scale), r = __frcp_rn(s);
+  uint32_t word = 0;
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    const float d = x[n] - lo, q0 = d * r;
+    const float q = fmaf(fmaf(-q0, s, d), r, q0);
+    word += (__float_as_uint(q + 12582912.f) & 15u) << (4 * n);
+  }
+  return make_uint2(word, pair_of(bits16(scale), bits16(from_float<T>(lo))));
 }
 
 }  // namespace aeg

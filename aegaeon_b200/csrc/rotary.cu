@@ -92,28 +92,37 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
     turn_per_pos = static_cast<double>(p.inv_freq[tid]) * 0.15915494309189535;  // 1 / (2 pi)
     pos += static_cast<int64_t>((p.axis[tid >> 4] >> (2 * (tid & 15))) & 3u) * p.axis_stride;
   }
+  // A thread's vectors: item k is head k / per_head, vector k % per_head of it, `off` elements into the
+  // token's row of queries or keys.
+  auto locate = [&](int k, int per, int base, int& which, int& c) {
+    const int head = k / per;
+    c = k - head * per;
+    which = head >= p.heads[0] ? 1 : 0;
+    return (which ? head - p.heads[0] : head) * p.dim + base + c * kVec;
+  };
+  auto source = [&](int which, int64_t t, int off) {
+    return reinterpret_cast<const V*>((which ? p.x[1] : p.x[0]) + t * (which ? p.x_stride[1] : p.x_stride[0]) + off);
+  };
+  auto target = [&](int which, int64_t t, int off) {
+    return reinterpret_cast<V*>((which ? p.out[1] : p.out[0]) + t * (which ? p.out_stride[1] : p.out_stride[0]) + off);
+  };
+  // The first item of the next token and its position are loaded while this one is rotated.
+  int which0 = 0, c0 = 0;
+  const int off0 = tid < n_rot ? locate(tid, per_head, 0, which0, c0) : 0;
+  V a0{}, b0{};
+  int64_t at = 0;
+  auto load_first = [&](int64_t t) {
+    if (t >= p.tokens) return;
+    if (tid < n_rot) {
+      const V* src = source(which0, t, off0);
+      a0 = src[0];
+      b0 = src[per_head];
+    }
+    if (tid < p.half) at = pos[t];
+  };
+  load_first(blockIdx.x);
   int buf = 0;
   for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x, buf ^= 1) {
-    const int64_t at = tid < p.half ? pos[t] : 0;
-    // This thread's vectors: item k is head k / per_head, vector k % per_head. The first one is
-    // loaded before the angles are made.
-    auto locate = [&](int k, int per, int base, const V*& src, V*& dst) {
-      const int head = k / per, c = k - head * per;
-      const int which = head >= p.heads[0] ? 1 : 0;
-      const int64_t off = static_cast<int64_t>(which ? head - p.heads[0] : head) * p.dim + base + c * kVec;
-      src = reinterpret_cast<const V*>((which ? p.x[1] : p.x[0]) + t * (which ? p.x_stride[1] : p.x_stride[0]) + off);
-      dst = reinterpret_cast<V*>((which ? p.out[1] : p.out[0]) + t * (which ? p.out_stride[1] : p.out_stride[0]) + off);
-      return c;
-    };
-    const V* src = nullptr;
-    V* dst = nullptr;
-    V a{}, b{};
-    int c = 0;
-    if (tid < n_rot) {
-      c = locate(tid, per_head, 0, src, dst);
-      a = src[0];
-      b = src[per_head];
-    }
     if (tid < p.half) {
       const double turn = turn_per_pos * static_cast<double>(at);
       float sn, cs;
@@ -121,12 +130,16 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
       s_cos[buf][tid] = cs * p.scaling;
       s_sin[buf][tid] = sn * p.scaling;
     }
+    V a = a0, b = b0;
+    load_first(t + gridDim.x);
     // One barrier a token: the buffers alternate, and a thread passes the next token's barrier only
     // when all threads have left this token's rotations behind.
     __syncthreads();
+    int which = which0, c = c0, off = off0;
     for (int k = tid; k < n_rot; k += kThreads) {
       if (k != tid) {
-        c = locate(k, per_head, 0, src, dst);
+        off = locate(k, per_head, 0, which, c);
+        const V* src = source(which, t, off);
         a = src[0];
         b = src[per_head];
       }
@@ -139,12 +152,13 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
         oa[i] = fa[i] * cs - fb[i] * sn;
         ob[i] = fb[i] * cs + fa[i] * sn;
       }
+      V* dst = target(which, t, off);
       dst[0] = from_floats<T, kVec>(oa);
       dst[per_head] = from_floats<T, kVec>(ob);
     }
     for (int k = tid; k < n_rest; k += kThreads) {
-      locate(k, rest, 2 * p.half, src, dst);
-      dst[0] = src[0];
+      off = locate(k, rest, 2 * p.half, which, c);
+      target(which, t, off)[0] = source(which, t, off)[0];
     }
   }
 }

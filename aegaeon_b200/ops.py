@@ -680,7 +680,7 @@ def rotary_multi_axis(query: torch.Tensor, key: torch.Tensor, positions: torch.T
     are dims (i, i + half); dims from ``2 * half`` on are copied. ``scaling`` multiplies the rotated
     dims. Returns new tensors unless ``query_out``/``key_out`` are given; those may be the inputs.
     """
-    T, Hq, D = q_shape = _token_rows(query, "query", "[T, Hq, D]")
+    T, Hq, D = _token_rows(query, "query", "[T, Hq, D]")
     k_shape = _token_rows(key, "key", "[T, Hkv, D]")
     dtype = query.dtype
     if dtype not in _DTYPES or key.dtype != dtype:
@@ -707,11 +707,11 @@ def rotary_multi_axis(query: torch.Tensor, key: torch.Tensor, positions: torch.T
     for name, t in (("key", key), ("positions", positions), ("inv_freq", inv_freq)):
         _on_device(index, t, name)
     if query_out is None:
-        query_out = torch.empty(q_shape, dtype=dtype, device=query.device)
+        query_out = torch.empty_like(query, memory_format=torch.contiguous_format)
     else:
         _check_rotary_out(index, query_out, query, "query_out")
     if key_out is None:
-        key_out = torch.empty(k_shape, dtype=dtype, device=key.device)
+        key_out = torch.empty_like(key, memory_format=torch.contiguous_format)
     else:
         _check_rotary_out(index, key_out, key, "key_out")
     _launch(index, "rotary_multi_axis", lib.aeg_rotary_multi_axis, query_out.data_ptr(), query_out.stride(0),
