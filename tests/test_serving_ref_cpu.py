@@ -115,6 +115,32 @@ def test_int4_calls_refuse_on_the_host():
         assert call(n=-1) == INVAL
 
 
+def test_int4_attention_refuses_on_the_host():
+    p, _k = _aligned()
+    lib = _native.lib
+    need = lib.aeg_decode_workspace_size(2, 8, 2, 128)
+    assert lib.aeg_decode_plan_int4(p, need, p, 4, p, 2, 8, 2, 64, None) == UNSUP
+    assert lib.aeg_decode_plan_int4(p, need, p, 4, p, 2, 34, 2, 128, None) == INVAL
+    assert lib.aeg_decode_plan_int4(p + 8, need, p, 4, p, 2, 8, 2, 128, None) == INVAL
+    assert lib.aeg_decode_plan_int4(p, need - 1, p, 4, p, 2, 8, 2, 128, None) == INVAL
+    assert lib.aeg_decode_plan_int4(p, need, None, 4, p, 2, 8, 2, 128, None) == INVAL
+    good = dict(o=p, os=1024, q=p, qs=1024, c=p, bs=2 * 1152, n=8, t=p, W=4, sl=p, B=2, Hq=8, Hkv=2, D=128, dt=0, ws=p, wsb=need, f=0)
+
+    def call(**kw):
+        a = dict(good, **kw)
+        return lib.aeg_paged_attn_decode_int4(a["o"], a["os"], a["q"], a["qs"], a["c"], a["bs"], a["n"], a["t"], a["W"], a["sl"],
+                                              a["B"], a["Hq"], a["Hkv"], a["D"], 0.1, a["dt"], a["ws"], a["wsb"], a["f"], None)
+
+    assert call(B=0) == 0 and call(B=-1) == INVAL
+    assert call(D=64) == UNSUP and call(Hq=9) == INVAL and call(Hq=34) == INVAL and call(dt=3) == INVAL and call(W=0) == INVAL
+    assert call(o=None) == INVAL and call(q=None) == INVAL and call(c=None) == INVAL and call(t=None) == INVAL and call(sl=None) == INVAL
+    assert call(os=1000) == INVAL and call(qs=1000) == INVAL and call(qs=1025) == INVAL and call(q=p + 2) == INVAL and call(o=p + 1) == INVAL
+    assert call(bs=2 * 1152 - 8) == INVAL and call(bs=2 * 1152 + 4) == INVAL and call(c=p + 8) == INVAL
+    assert call(n=0) == INVAL and call(n=1 << 31) == INVAL
+    assert call(ws=None) == INVAL and call(ws=p + 16) == INVAL and call(wsb=need - 1) == INVAL
+    assert call(f=2) == INVAL and call(f=4) == INVAL
+
+
 def test_rotary_refuses_on_the_host():
     p, _k = _aligned()
     lib = _native.lib
