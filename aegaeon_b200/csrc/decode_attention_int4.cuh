@@ -152,11 +152,35 @@ struct Int4Worker {
   }
 };
 
+// A worker's range of units and its first unit's record; an empty range if the plan does not fit this
+// launch. `report` says whether the caller reports that.
+struct Int4Range {
+  int u_beg, u_end;
+  int4 ra, rb;
+};
+__device__ __forceinline__ Int4Range int4_range(const AttnParams& p, int gw, int total_warps, bool report) {
+  const uint64_t keep = l2_policy_evict_last();
+  Int4Range r;
+  r.u_beg = ld_hint(&p.ws.warp_rec[3 * gw].x, keep);
+  r.ra = ld_hint(&p.ws.warp_rec[3 * gw + 1], keep);
+  r.rb = ld_hint(&p.ws.warp_rec[3 * gw + 2], keep);
+  r.u_end = ld_hint(&p.ws.warp_rec[3 * (gw + 1)].x, keep);
+  const int planned_warps = ld_hint(&p.ws.header[kHdrWarps], keep);
+  const int planned_units = ld_hint(&p.ws.header[kHdrUnits], keep);
+  if (!(planned_warps == total_warps && planned_units <= p.max_units && r.u_beg >= 0 && r.u_beg <= r.u_end &&
+        r.u_end <= planned_units)) {
+    if (report && r.u_beg != r.u_end) atomicOr(&g_deverr_attn, AEG_DEVERR_PLAN_MISMATCH);
+    r.u_end = r.u_beg;
+  }
+  return r;
+}
+
 // The requesting warp: lane w walks worker w's units (their records and queries) and tiles. Block ids
 // come four at a time and four tiles ahead, unit records one unit ahead, so that no step waits for a
 // load it has just made (with ids two tiles ahead every step did, and streaming took 1.1 to 1.2 times
-// as long). Without a tensor map there is no zero fill: a tile whose id
-// is outside the pool is not fetched and has no valid tokens.
+// as long). A worker's first unit's record and queries are not among them: the worker fetches those
+// itself, beside the first tiles. Without a tensor map there is no zero fill: a tile whose id is
+// outside the pool is not fetched and has no valid tokens.
 template <typename T, int NT>
 __device__ __forceinline__ void request_tiles(const AttnParams& p, uint8_t* smem, int lane) {
   using SL = Int4Smem<NT>;
@@ -165,31 +189,20 @@ __device__ __forceinline__ void request_tiles(const AttnParams& p, uint8_t* smem
   const Int4Worker<NT> w(smem, worker ? lane : 0);
   const int gw = static_cast<int>(blockIdx.x) * SL::kWarps + (worker ? lane : 0);
 
-  int u_beg = 0, u_end = 0, planned_warps = 0, planned_units = 0;
-  int4 ra, rb;
-  auto load_plan = [&]() {
-    u_beg = ld_hint(&p.ws.warp_rec[3 * gw].x, keep);
-    ra = ld_hint(&p.ws.warp_rec[3 * gw + 1], keep);
-    rb = ld_hint(&p.ws.warp_rec[3 * gw + 2], keep);
-    u_end = ld_hint(&p.ws.warp_rec[3 * (gw + 1)].x, keep);
-    planned_warps = ld_hint(&p.ws.header[kHdrWarps], keep);
-    planned_units = ld_hint(&p.ws.header[kHdrUnits], keep);
-  };
   // The plan and the first tiles come before the wait for the preceding kernel only where the host
   // knows that it wrote neither.
   const bool early = p.plan_ready && p.prefetch_kv;
-  if (p.plan_ready) load_plan();
+  const int total_warps = static_cast<int>(gridDim.x) * SL::kWarps;
+  Int4Range range;
+  if (p.plan_ready) range = int4_range(p, gw, total_warps, worker);
   if (!early) pdl_wait_primary();
-  if (!p.plan_ready) load_plan();
-  if (!(planned_warps == static_cast<int>(gridDim.x) * SL::kWarps && planned_units <= p.max_units && u_beg >= 0 &&
-        u_beg <= u_end && u_end <= planned_units)) {
-    if (worker && u_beg != u_end) atomicOr(&g_deverr_attn, AEG_DEVERR_PLAN_MISMATCH);
-    u_end = u_beg;
-  }
+  if (!p.plan_ready) range = int4_range(p, gw, total_warps, worker);
+  const int u_end = range.u_end;
+  int4 ra = range.ra, rb = range.rb;
 
   // Tiles: unit ut (its record in ra, rb), tile i of n, the ids of the tiles from i on that are at hand
   // (the first `at_hand` of c) and those after them (d); the next unit's record.
-  int ut = u_beg, i = 0, n = 0, n_ctx = 0, at_hand = 0;
+  int ut = range.u_beg, i = 0, n = 0, n_ctx = 0, at_hand = 0;
   int4 c = make_int4(0, 0, 0, 0), d = c;
   const int* ids = p.tables;  // of the first tile in d
   const T* tiles = static_cast<const T*>(p.k_cache);
@@ -216,10 +229,10 @@ __device__ __forceinline__ void request_tiles(const AttnParams& p, uint8_t* smem
       }
     }
   };
-  // Queries: unit uq, its record.
-  int uq = u_beg;
-  int4 qa = ra, qb = rb;
   enter();
+  // Queries: unit uq, its record (that of the second unit, the first one's being the worker's own).
+  int uq = ut + 1;
+  int4 qa = na, qb = nb;
 
   uint32_t st = 0, ph = 1, qph = 1;  // a barrier that has completed no phase counts as free
   auto tile_step = [&]() -> bool {
@@ -351,8 +364,11 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
   T* out = static_cast<T*>(p.out);
   const int quad = lane & 3;  // column pair of the accumulator fragment
   const int grp = lane >> 2;  // row of the accumulator fragment
+  Int4Range range;
+  if (p.plan_ready) range = int4_range(p, gw, total_warps, false);
   pdl_wait_primary();
   pdl_launch_dependents();
+  if (!p.plan_ready) range = int4_range(p, gw, total_warps, false);
 
   // This warp's share of the split merge and the launches with this plan so far (see
   // decode_attn_kernel); needed when its units are done.
@@ -372,13 +388,32 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
   };
   uint32_t st_con = 0, ph_con = 0, q_phase = 0;
 
+  // The first unit's record comes from the plan and its queries from global memory; later ones through
+  // shared memory, from the requesting warp.
+  bool first = range.u_beg < range.u_end;
   while (!lost) {
-    wait(wk.qfull, q_phase);
-    if (lost) break;
-    q_phase ^= 1;
-    const int4 rec = *wk.record;
-    const int n = rec.x, slot = rec.y, b = rec.z, h = rec.w;
-    if (n < 0) break;
+    int n, slot, b, h;
+    if (first) {
+      n = unit_items(range.ra, range.rb, p);
+      slot = range.ra.w;
+      b = range.ra.x / p.Hkv;
+      h = range.ra.x % p.Hkv;
+      if (n == 0) {
+        if (lane == 0) atomicOr(&g_deverr_attn, AEG_DEVERR_PLAN_MISMATCH);
+        first = false;
+        continue;
+      }
+    } else {
+      wait(wk.qfull, q_phase);
+      if (lost) break;
+      q_phase ^= 1;
+      const int4 rec = *wk.record;
+      n = rec.x;
+      slot = rec.y;
+      b = rec.z;
+      h = rec.w;
+      if (n < 0) break;
+    }
 
     // A negative scale goes into the sign of q, so that larger sums always mean larger scores. bf16
     // queries go to fp16 exactly after a power of two of the head's own (elements below 2^-17 of the
@@ -395,12 +430,17 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (head < G && p.q_bulk) {
-          x = lds128(wk.q + head * (kHeadDim * 2) + w * 64 + quad * 16);
-        } else if (head < G) {  // rows that are not 16-byte aligned
-          const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + static_cast<int64_t>(b) * p.q_stride +
-                                                                  (static_cast<int64_t>(h) * G + head) * kHeadDim + w * 32 + quad * 8);
-          x = make_uint4(src[0], src[1], src[2], src[3]);
+        const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(b) * p.q_stride +
+                       (static_cast<int64_t>(h) * G + head) * kHeadDim + w * 32 + quad * 8;
+        if (head < G) {
+          if (!p.q_bulk) {  // rows that are not 16-byte aligned
+            const uint32_t* s4 = reinterpret_cast<const uint32_t*>(src);
+            x = make_uint4(s4[0], s4[1], s4[2], s4[3]);
+          } else if (first) {
+            x = *reinterpret_cast<const uint4*>(src);
+          } else {
+            x = lds128(wk.q + head * (kHeadDim * 2) + w * 64 + quad * 16);
+          }
         }
         xw[w][0] = x.x ^ flip;
         xw[w][1] = x.y ^ flip;
@@ -451,7 +491,7 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
       sc[nt][1] = __shfl_sync(0xffffffffu, back, 8 * quad + 4);
     }
     // The slot is free once every lane's values have arrived: a vote on them needs them all.
-    {
+    if (!first) {
       uint32_t dep = 0;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -460,6 +500,7 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
       const uint32_t any = __ballot_sync(0xffffffffu, dep != 0);
       if (lane == 0) mbar_arrive_after(wk.qempty, any);
     }
+    first = false;
 
     // Running maximum of the unscaled scores, that times the scale, and the score from which it moves;
     // sum of p; sum of p * (minimum + middle * scale) [column][group]; sum of the rounded P * scale
@@ -672,7 +713,7 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
           om[nt][i][1] += __shfl_xor_sync(0xffffffffu, om[nt][i][1], off);
         }
     fold();
-    const float unit_o = 1.f / vmul;
+    const float unit_o = __uint_as_float((254u << 23) - __float_as_uint(vmul));  // 1 / vmul, a power of two
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -688,7 +729,7 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
             y[2 * j + 1] = fmaf(o[4 * g + j][nt][i + 2], unit_o, om[nt][i][g]);
           }
           if (slot < 0) {
-            const float inv = l[nt][i] > 0.f ? 1.f / l[nt][i] : (l[nt][i] == 0.f ? 0.f : l[nt][i]);
+            const float inv = l[nt][i] == 0.f ? 0.f : __frcp_rn(l[nt][i]);
             T* dst = out + static_cast<int64_t>(b) * p.out_stride + (static_cast<int64_t>(h) * G + head) * kHeadDim + 64 * g +
                      8 * grp;
             if (aligned(dst, 16)) {
