@@ -273,9 +273,24 @@ __device__ __forceinline__ long long block_excl_scan64(long long v, long long* s
   return off + incl - v;
 }
 
+// With kScan the kernel stops after the scans and leaves what the lists are written from to
+// plan_lists_kernel: this one CTA spent most of its time writing them (two sequences of 32,768 tokens:
+// 25 us in all, of them 1,600 units behind their block-table loads).
+struct PlanScan {  // in the (still unused) partial-result area: one per pair, behind the totals
+  long long items;        // cost-axis positions; -1: nothing planned
+  long long merge_items;
+  int units, entries, slots, pad;
+};
+struct PlanPair {
+  long long o, mo;  // position of the pair's first virtual item; first merge item
+  int u, sp, slot, pad;
+};
+static_assert(sizeof(PlanScan) == 32 && sizeof(PlanPair) == 32, "16-byte aligned records");
+
+template <bool kScan>
 __global__ void __launch_bounds__(kPlanThreads, 1)
 decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tables, int B, int Hkv,
-                   int G, int table_stride, int W, WsPtrs ws) {
+                   int G, int table_stride, int W, WsPtrs ws, PlanScan* scan) {
   __shared__ long long s_red[kPlanThreads / 32];
   __shared__ int s_warp[kPlanThreads / 32];
   __shared__ int s_nb[kPlanCachedSeqs];  // blocks per sequence (first kPlanCachedSeqs sequences)
@@ -284,6 +299,7 @@ decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tab
   __shared__ int s_long_ofs[kPlanLongPairs + 1];  // prefix sums of the pairs' unit counts
   __shared__ int s_nlong;
   const int tid = threadIdx.x;
+  if constexpr (kScan) pdl_launch_dependents();
   if (tid == 0) s_nlong = 0;
   const int P = B * Hkv;
   const int cap = table_stride * kBlockTokens;
@@ -311,6 +327,7 @@ decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tab
       ws.header[kHdrWarps] = W;
       ws.header[kHdrUnits] = 0;
       ws.header[kHdrSplitPairs] = 0;
+      if constexpr (kScan) scan->items = -1;
     }
     for (int w = tid; w <= W; w += kPlanThreads) ws.warp_rec[3 * w] = make_int4(0, 0, 0, 0);
     for (int w = tid; w < W; w += kPlanThreads) ws.merge_rec[w] = make_int4(0, 0, 0, 0);
@@ -368,6 +385,26 @@ decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tab
     ws.header[kHdrSplitPairs] = S;
     ws.header[kHdrSlots] = SL;
     ws.header[kHdrMergeItems] = static_cast<int>(MI < 0x7fffffffLL ? MI : 0x7fffffffLL);
+  }
+  if constexpr (kScan) {
+    if (tid == 0) *scan = PlanScan{I, MI, U, S, SL, 0};
+    PlanPair* pairs = reinterpret_cast<PlanPair*>(scan + 1);
+    o = o_t;
+    for (int p = p0; p < p1; ++p) {
+      const int nb = blocks_of(p / Hkv);
+      pairs[p] = PlanPair{o, mo, u, sp, slot, 0};
+      const int c = nb > 0 ? cuts(o + kUnitCost, nb) : 0;
+      if (nb == 0 || c > 0) {
+        ++sp;
+        mo += merge_items(merge_shape(nb == 0 ? 0 : c + 1, G), G);
+      }
+      if (nb > 0) {
+        u += c + 1;
+        if (c > 0) slot += c + 1;
+        o += nb + kUnitCost;
+      }
+    }
+    return;
   }
   for (int c = tid; c < W; c += kPlanThreads) ws.warp_flag[c * kFlagStride] = 0;
   for (int w = Wp + tid; w <= W; w += kPlanThreads) ws.warp_rec[3 * w] = make_int4(U, 0, 0, 0);  // empty ranges
@@ -455,6 +492,70 @@ decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tab
     const int4 L = s_long[lo];
     const int k = t - s_long_ofs[lo];
     emit_unit(L.x, s_long_o[lo], blocks_of(L.x / Hkv), L.z, k, L.y + k, L.w + k);
+  }
+}
+
+// The lists of a plan from its scans, as decode_plan_kernel<false> writes them: a CTA a pair, a thread a
+// unit (and a worker's share of the pair's merge items).
+constexpr int kListThreads = 64;
+__global__ void __launch_bounds__(kListThreads)
+plan_lists_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tables, int B, int Hkv, int G, int table_stride,
+                  int W, WsPtrs ws, const PlanScan* scan) {
+  pdl_wait_primary();
+  const int tid = threadIdx.x;
+  const long long I = scan->items, MI = scan->merge_items;
+  if (I < 0) return;
+  const int U = scan->units, S = scan->entries;
+  const PlanPair* pairs = reinterpret_cast<const PlanPair*>(scan + 1);
+  const int Wp = I < W ? static_cast<int>(I) : W;
+  const int Wm = MI < W ? static_cast<int>(MI) : W;
+  const int cap = table_stride * kBlockTokens, P = B * Hkv;
+  for (int w = blockIdx.x * kListThreads + tid; w <= W; w += gridDim.x * kListThreads) {
+    if (w < W) ws.warp_flag[w * kFlagStride] = 0;
+    if (w >= Wp) ws.warp_rec[3 * w] = make_int4(U, 0, 0, 0);
+    if (w >= Wm && w < W) ws.merge_rec[w] = make_int4(S, 0, 0, 0);
+  }
+  const EqualCuts wk(I, Wp), mk(MI, Wm);
+  for (int p = blockIdx.x; p < P; p += gridDim.x) {
+    const PlanPair r = pairs[p];
+    const int b = p / Hkv;
+    const int n_ctx = min(max(seq_lens[b], 0), cap);
+    const int nb = (n_ctx + kBlockTokens - 1) / kBlockTokens;
+    const long long ob = r.o + kUnitCost;
+    const int c = nb > 0 ? static_cast<int>(wk.le(ob + nb - 1) - wk.le(ob)) : 0;
+    if (nb == 0 || c > 0) {
+      const int shape = merge_shape(nb == 0 ? 0 : c + 1, G), n_it = merge_items(shape, G);
+      if (tid == 0) {
+        const int w0 = nb > 0 ? static_cast<int>(wk.le(ob) - 1) : 0;
+        const int w1 = nb > 0 ? static_cast<int>(wk.le(ob + nb - 1) - 1) : 0;
+        ws.split_pairs[r.sp] = nb == 0 ? make_int4(p, 0, shape << 16, 0)
+                                       : make_int4(p, r.slot, (c + 1) | (shape << 16), w0 | ((w1 - w0 + 1) << 16));
+      }
+      const long long w_hi = mk.le(r.mo + n_it - 1);
+      for (long long w = mk.le(r.mo - 1) + tid; w < w_hi; w += kListThreads) {
+        const long long st = mk.start(w);
+        const long long en = w + 1 < Wm ? mk.start(w + 1) : MI;
+        ws.merge_rec[w] = make_int4(r.sp, static_cast<int>(st - r.mo), static_cast<int>(en - st), 0);
+      }
+    }
+    if (nb == 0) continue;
+    const long long wc = wk.le(ob);  // first worker starting after the pair's first block
+    for (int k = tid; k <= c; k += kListThreads) {
+      const long long xa = k == 0 ? ob : wk.start(wc + k - 1);
+      const long long xb = k == c ? ob + nb : wk.start(wc + k);
+      const int j0 = static_cast<int>(xa - ob), j1 = static_cast<int>(xb - ob), n = j1 - j0;
+      const int* tb = tables + static_cast<int64_t>(b) * table_stride + j0;
+      const int4 ra = make_int4(p, j0, j1, c > 0 ? r.slot + k : -1);
+      const int4 rb = make_int4(n_ctx, tb[0], n > 1 ? tb[1] : 0, n > 2 ? tb[2] : 0);
+      ws.units[2 * (r.u + k)] = ra;
+      ws.units[2 * (r.u + k) + 1] = rb;
+      const long long w_hi = wk.le(xa);
+      for (long long w = wk.le((k == 0 ? r.o : xa) - 1); w < w_hi; ++w) {
+        ws.warp_rec[3 * w] = make_int4(r.u + k, 0, 0, 0);
+        ws.warp_rec[3 * w + 1] = ra;
+        ws.warp_rec[3 * w + 2] = rb;
+      }
+    }
   }
 }
 
@@ -1762,6 +1863,33 @@ int decode_int4(void* out, int64_t out_stride, const void* q, int64_t q_stride, 
   return st;
 }
 
+// Plans on `stream`: scans in one CTA, then the lists over the GPU where the pairs' records fit the
+// partial-result area; else (far more pairs than workers) all of it in one CTA.
+int launch_plan(const char* what, const int32_t* seq_lens, const int32_t* block_tables, int B, int Hkv, int G,
+                int table_stride, int W, void* workspace, const WsLayout& L, cudaStream_t stream) {
+  const WsPtrs ws = ws_ptrs(workspace, L);
+  PlanScan* scan = reinterpret_cast<PlanScan*>(ws.part_ml);
+  const int64_t P = int64_t(B) * Hkv;
+  if (P == 0 || sizeof(PlanScan) + sizeof(PlanPair) * P > L.total - L.part_ml) {
+    decode_plan_kernel<false><<<1, kPlanThreads, 0, stream>>>(seq_lens, block_tables, B, Hkv, G, table_stride, W, ws, scan);
+    AEG_CHECK_LAUNCH(what);
+    return AEG_OK;
+  }
+  decode_plan_kernel<true><<<1, kPlanThreads, 0, stream>>>(seq_lens, block_tables, B, Hkv, G, table_stride, W, ws, scan);
+  AEG_CHECK_LAUNCH(what);
+  cudaLaunchAttribute attr[1] = {pdl_attr()};
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(P < int64_t(num_sms()) * 16 ? P : int64_t(num_sms()) * 16));
+  cfg.blockDim = dim3(kListThreads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  AEG_CHECK_CUDA(cudaLaunchKernelEx(&cfg, plan_lists_kernel, static_cast<const int*>(seq_lens),
+                                    static_cast<const int*>(block_tables), B, Hkv, G, table_stride, W, ws,
+                                    static_cast<const PlanScan*>(scan)));
+  return AEG_OK;
+}
+
 int plan_common(const char* what, void* workspace, size_t workspace_bytes, const int32_t* block_tables, int table_stride,
                 const int32_t* seq_lens, int B, int Hq, int Hkv, int D, bool int4, void* stream) {
   int st = validate_shape(B, Hq, Hkv, D, table_stride);
@@ -1774,9 +1902,9 @@ int plan_common(const char* what, void* workspace, size_t workspace_bytes, const
   const int W = int4 ? worker_warps_int4(Hq / Hkv) : worker_warps(Hq / Hkv);
   if (W > L.max_warps)
     return set_error(AEG_ERR_UNSUPPORTED, "%s: %d worker warps exceed the workspace's %d", what, W, L.max_warps);
-  decode_plan_kernel<<<1, kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(seq_lens, block_tables, B, Hkv, Hq / Hkv,
-                                                                                 table_stride, W, ws_ptrs(workspace, L));
-  AEG_CHECK_LAUNCH(what);
+  const int launched = launch_plan(what, seq_lens, block_tables, B, Hkv, Hq / Hkv, table_stride, W, workspace, L,
+                                   static_cast<cudaStream_t>(stream));
+  if (launched != AEG_OK) return launched;
   mark_plan_fresh(workspace);
   return AEG_OK;
 }
@@ -1938,9 +2066,8 @@ int aeg_paged_attn_decode_noalloc(void* out, int64_t out_stride, const void* q, 
   bool waited = false;
   st = order.enter(s, &waited);
   if (st != AEG_OK) return st;
-  aeg::decode_plan_kernel<<<1, aeg::kPlanThreads, 0, s>>>(seq_lens, block_tables, B, Hkv, Hq / Hkv, table_stride, W,
-                                                          aeg::ws_ptrs(scratch, L));
-  AEG_CHECK_LAUNCH("decode_plan (noalloc)");
+  st = aeg::launch_plan("decode_plan (noalloc)", seq_lens, block_tables, B, Hkv, Hq / Hkv, table_stride, W, scratch, L, s);
+  if (st != AEG_OK) return st;
   dl.prm.plan_ready = 0;  // the plan kernel directly precedes this launch: read it after the wait
   return aeg::decode_launch(dl, s, order);
 }
