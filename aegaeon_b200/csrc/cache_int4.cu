@@ -81,31 +81,51 @@ __global__ void __launch_bounds__(kThreads) write_int4_kernel(const Rows p) {
       if (k % kHeads == 0) slot[k / kHeads] = t < p.tokens ? p.slots[t] : -1;
       v[k] = there ? load8<kVec>(rows + t * stride + (k % kHeads) * kInt4Dim) : make_uint4(0u, 0u, 0u, 0u);
     }
+    // Tokens of one word pair (an even slot and the next one) are stored together: 4-byte words of both
+    // instead of 2-byte halves of each.
+    bool pair = kTokens % 2 == 0;
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      float x[8];
-      const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const float2 f = unpack2<T>(w[n]);
-        x[2 * n] = f.x;
-        x[2 * n + 1] = f.y;
-      }
-      const uint2 q = int4_quantise<T>(x);
-      const int64_t s = slot[k / kHeads];
-      if (s >= p.num_slots) {
+    for (int j = 0; j < kTokens; ++j) {
+      if (slot[j] >= p.num_slots) {
         if (lane == 0) atomicOr(&g_deverr_int4, AEG_DEVERR_SLOT_RANGE);
-      } else if (s >= 0 && h0 + k % kHeads < p.heads) {
-        const int t = static_cast<int>(s & 15);
-        uint8_t* tile = tiles + (s >> 4) * p.block_stride + (k % kHeads) * kInt4TileBytes;
-        if (is_key) {
-          *reinterpret_cast<uint32_t*>(tile + int4_key_word(t, l)) = q.x;
-        } else {
-          uint16_t* half = reinterpret_cast<uint16_t*>(tile + int4_value_half(t, l));
-          half[0] = static_cast<uint16_t>(q.x);
-          half[2] = static_cast<uint16_t>(q.x >> 16);
+        slot[j] = -1;
+      }
+      if (j % 2) pair = pair && slot[j - 1] >= 0 && !(slot[j - 1] & 1) && slot[j] == slot[j - 1] + 1;
+    }
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      if (h0 + i >= p.heads) break;
+      uint2 q[kTokens];
+#pragma unroll
+      for (int j = 0; j < kTokens; ++j) {
+        float x[8];
+        const uint4& u = v[j * kHeads + i];
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const float2 f = unpack2<T>(w[n]);
+          x[2 * n] = f.x;
+          x[2 * n + 1] = f.y;
         }
-        if ((l & 7) == 0) *reinterpret_cast<uint32_t*>(tile + pairs_at + t * 8) = q.y;
+        q[j] = int4_quantise<T>(x);
+      }
+#pragma unroll
+      for (int j = 0; j < kTokens; ++j) {
+        if (slot[j] < 0) continue;
+        const int t = static_cast<int>(slot[j] & 15);
+        uint8_t* tile = tiles + (slot[j] >> 4) * p.block_stride + i * kInt4TileBytes;
+        if ((l & 7) == 0) *reinterpret_cast<uint32_t*>(tile + pairs_at + t * 8) = q[j].y;
+        if (!pair) {
+          // A key lane's word as two halves beside each other, a value lane's 4 bytes apart.
+          uint16_t* half = reinterpret_cast<uint16_t*>(tile + (is_key ? int4_key_word(t, l) : int4_value_half(t, l)));
+          half[0] = static_cast<uint16_t>(q[j].x);
+          half[is_key ? 1 : 2] = static_cast<uint16_t>(q[j].x >> 16);
+        } else if (j % 2 == 0) {
+          const uint32_t a = q[j].x, b = q[(j + 1) % kTokens].x;
+          uint32_t* word = reinterpret_cast<uint32_t*>(tile + (is_key ? int4_key_word(t, l) : int4_value_half(t, l)));
+          word[0] = is_key ? a : __byte_perm(a, b, 0x5410);
+          word[is_key ? 16 : 1] = is_key ? b : __byte_perm(a, b, 0x7632);  // the next token's key row is 64 bytes on
+        }
       }
     }
   }
@@ -140,12 +160,10 @@ __global__ void __launch_bounds__(kThreads) gather_int4_kernel(const Rows p) {
       if (s >= 0 && s < p.num_slots && h0 + k % kHeads < p.heads) {
         const int t = static_cast<int>(s & 15);
         const uint8_t* tile = tiles + (s >> 4) * p.block_stride + (k % kHeads) * kInt4TileBytes;
-        if (is_key) {
-          word[k] = *reinterpret_cast<const uint32_t*>(tile + int4_key_word(t, l));
-        } else {
-          const uint16_t* half = reinterpret_cast<const uint16_t*>(tile + int4_value_half(t, l));
-          word[k] = half[0] | (uint32_t(half[2]) << 16);
-        }
+        // The 8 bytes around a key lane's word, or a value lane's two words with both tokens' halves.
+        const int at = is_key ? int4_key_word(t, l) : int4_value_half(t, l);
+        const uint2 two = *reinterpret_cast<const uint2*>(tile + (at & ~7));
+        word[k] = is_key ? (at & 4 ? two.y : two.x) : __byte_perm(two.x, two.y, t & 1 ? 0x7632 : 0x5410);
         pair[k] = *reinterpret_cast<const uint32_t*>(tile + pairs_at + t * 8);
       }
     }
@@ -201,15 +219,15 @@ Kernel pick(bool write, bool vec) {
   return vec ? gather_int4_kernel<T, true, kTokens, kHeads> : gather_int4_kernel<T, false, kTokens, kHeads>;
 }
 
-// Several (token, head) a warp only where every resident warp has as many; then 4, of one token where it
-// has 4 heads.
+// Several (token, head) a warp only where every resident warp has as many; then 4, of two tokens (which
+// often share their words) where there are 2 heads.
 template <typename T>
 Kernel pick(bool write, bool vec, int64_t items, int heads, int* tokens, int* chunk) {
   const bool many = items >= int64_t(num_sms()) * 16 * kWarpsPerCta;
-  *chunk = !many || heads == 1 ? 1 : (heads < 4 ? 2 : 4);
+  *chunk = !many || heads == 1 ? 1 : 2;
   *tokens = many ? 4 / *chunk : 1;
   if (!many) return pick<T, 1, 1>(write, vec);
-  return heads == 1 ? pick<T, 4, 1>(write, vec) : (heads < 4 ? pick<T, 2, 2>(write, vec) : pick<T, 1, 4>(write, vec));
+  return heads == 1 ? pick<T, 4, 1>(write, vec) : pick<T, 2, 2>(write, vec);
 }
 
 int launch(const char* what, bool write, const Rows& p, int dtype, cudaStream_t stream) {
@@ -224,8 +242,8 @@ int launch(const char* what, bool write, const Rows& p, int dtype, cudaStream_t 
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  const int64_t resident = std::max<int64_t>(int64_t(num_sms()) * 16 / chunks, 1);
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>((p.tokens + per_cta - 1) / per_cta, resident)),
+  const int64_t most = std::max<int64_t>(int64_t(num_sms()) * 256 / chunks, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>((p.tokens + per_cta - 1) / per_cta, most)),
                      static_cast<unsigned>(chunks));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
