@@ -23,7 +23,8 @@ __device__ unsigned int g_deverr_pool = 0;
 
 constexpr int kBlockTokens = 16;
 constexpr int kPlanThreads = 1024;
-constexpr int kScanPerThread = 4;
+constexpr int kScanRows = 8;  // rows of 32 counts a warp takes per step of a scan, all loads in flight
+constexpr int kScanStep = kPlanThreads * kScanRows;
 constexpr int kCopyThreads = 256;
 constexpr int kCopyUnroll = 8;
 constexpr int64_t kSegVecs = int64_t(kCopyThreads) * kCopyUnroll;  // 32 KiB a segment
@@ -82,6 +83,13 @@ __device__ __forceinline__ void copy_segment(const uint8_t* src, uint8_t* dst, i
     const int64_t end = min(begin + kSegVecs * 16, block_bytes);
     for (int64_t k = begin + threadIdx.x; k < end; k += kCopyThreads) dst[k] = src[k];
   }
+}
+
+// The counts of a warp's blocks b, b + 32, ... (b includes the lane); -1 past the end, which is neither
+// free nor live.
+__device__ __forceinline__ void load_counts(const int* ref_counts, int64_t b, int num_blocks, int (&rc)[kScanRows]) {
+#pragma unroll
+  for (int k = 0; k < kScanRows; ++k) rc[k] = b + 32 * k < num_blocks ? ref_counts[b + 32 * k] : -1;
 }
 
 struct PoolParams {
@@ -162,24 +170,31 @@ fork_plan_kernel(const PoolParams p, const int64_t* __restrict__ src, const int6
     if (need) ws.entry[i].w = want + rank;
     want += total;
   }
+  // The first `want` free blocks; the next step's counts are on their way while this one's are summed.
+  // A warp takes consecutive rows of 32, so that ballots rank them.
   int found = 0;
-  for (int b0 = 0; b0 < p.num_blocks && found < want; b0 += kPlanThreads * kScanPerThread) {
-    const int b = b0 + tid * kScanPerThread;
-    bool is_free[kScanPerThread];
+  const int lane = tid & 31;
+  const int64_t first = int64_t(tid >> 5) * 32 * kScanRows + lane;
+  int ahead[kScanRows];
+  if (want > 0) load_counts(p.ref_counts, first, p.num_blocks, ahead);
+  for (int64_t b0 = 0; b0 < p.num_blocks && found < want; b0 += kScanStep) {
+    uint32_t is_free[kScanRows];
     int mine = 0;
 #pragma unroll
-    for (int k = 0; k < kScanPerThread; ++k) {
-      is_free[k] = b + k < p.num_blocks && p.ref_counts[b + k] == 0;
-      mine += is_free[k];
+    for (int k = 0; k < kScanRows; ++k) {
+      is_free[k] = __ballot_sync(0xffffffffu, ahead[k] == 0);
+      mine += __popc(is_free[k]);
     }
+    load_counts(p.ref_counts, b0 + kScanStep + first, p.num_blocks, ahead);
     int total;
-    int rank = found + cta_scan(mine, s_warp, total);
+    int rank = found + cta_scan(lane == 0 ? mine : 0, s_warp, total);
+    rank = __shfl_sync(0xffffffffu, rank, 0);
 #pragma unroll
-    for (int k = 0; k < kScanPerThread; ++k)
-      if (is_free[k]) {
-        if (rank < want) ws.free_ids[rank] = b + k;
-        ++rank;
-      }
+    for (int k = 0; k < kScanRows; ++k) {
+      const int at = rank + __popc(is_free[k] & ((1u << lane) - 1));
+      if (((is_free[k] >> lane) & 1u) && at < want) ws.free_ids[at] = static_cast<int>(b0 + first) + 32 * k;
+      rank += __popc(is_free[k]);
+    }
     found += total;
   }
   __syncthreads();
@@ -284,40 +299,51 @@ compact_plan_kernel(const PoolParams p, CompactScratch ws, CompactOut out) {
   pdl_launch_dependents();
   pdl_wait_primary();
   const int tid = threadIdx.x;
+  const int lane = tid & 31;
+  const int64_t first = int64_t(tid >> 5) * 32 * kScanRows + lane;
+  int rc[kScanRows], ahead[kScanRows];
   int mine = 0, n_live = 0;
-  for (int b = tid; b < p.num_blocks; b += kPlanThreads) mine += p.ref_counts[b] > 0;
+  for (int64_t b0 = 0; b0 < p.num_blocks; b0 += kScanStep) {
+    load_counts(p.ref_counts, b0 + first, p.num_blocks, rc);
+#pragma unroll
+    for (int k = 0; k < kScanRows; ++k) mine += rc[k] > 0;
+  }
+  load_counts(p.ref_counts, first, p.num_blocks, ahead);
   cta_scan(mine, s_warp, n_live);
   // There are as many free ids below n_live as live ones from it on: listed in order of id, the
   // former fill the list's first half, the latter its second.
   int listed = 0;
-  for (int b0 = 0; b0 < p.num_blocks; b0 += kPlanThreads * kScanPerThread) {
-    const int b = b0 + tid * kScanPerThread;
-    int rc[kScanPerThread];
+  for (int64_t b0 = 0; b0 < p.num_blocks; b0 += kScanStep) {
+    const int64_t b = b0 + first;
+    uint32_t in_list[kScanRows];
     int count = 0;
 #pragma unroll
-    for (int k = 0; k < kScanPerThread; ++k) {
-      rc[k] = b + k < p.num_blocks ? p.ref_counts[b + k] : 0;
-      count += b + k < p.num_blocks && (b + k < n_live) == (rc[k] <= 0);
+    for (int k = 0; k < kScanRows; ++k) {
+      rc[k] = ahead[k];
+      const int64_t id = b + 32 * k;
+      in_list[k] = __ballot_sync(0xffffffffu, id < p.num_blocks && (id < n_live) == (rc[k] <= 0));
+      count += __popc(in_list[k]);
     }
+    load_counts(p.ref_counts, b + kScanStep, p.num_blocks, ahead);
     int total;
-    int at = listed + cta_scan(count, s_warp, total);
+    int at = listed + cta_scan(lane == 0 ? count : 0, s_warp, total);
+    at = __shfl_sync(0xffffffffu, at, 0);
 #pragma unroll
-    for (int k = 0; k < kScanPerThread; ++k) {
-      if (b + k >= p.num_blocks) break;
-      const bool low = b + k < n_live, live = rc[k] > 0;
-      if (low != live) ws.list[at++] = b + k;
-      out.remap[b + k] = live ? b + k : -1;
-      out.ref_counts[b + k] = low ? max(rc[k], 0) : 0;
+    for (int k = 0; k < kScanRows; ++k) {
+      const int id = static_cast<int>(b) + 32 * k;
+      if (b + 32 * k < p.num_blocks) {
+        const bool low = id < n_live, live = rc[k] > 0;
+        const int place = at + __popc(in_list[k] & ((1u << lane) - 1));
+        if (low != live) ws.list[place] = id;
+        // A moving block's place in the list until compact_apply_kernel puts its new id there.
+        out.remap[id] = !live ? -1 : (low ? id : -2 - place);
+        out.ref_counts[id] = low ? max(rc[k], 0) : 0;
+      }
+      at += __popc(in_list[k]);
     }
     listed += total;
   }
   const int moves = listed / 2;
-  __syncthreads();
-  for (int r = tid; r < moves; r += kPlanThreads) {
-    const int to = ws.list[r], from = ws.list[moves + r];
-    out.remap[from] = to;
-    out.ref_counts[to] = p.ref_counts[from];
-  }
   if (tid == 0) {
     ws.moves[0] = moves;
     out.num_live[0] = n_live;
@@ -329,6 +355,14 @@ __global__ void __launch_bounds__(kCopyThreads) compact_apply_kernel(const PoolP
   pdl_launch_dependents();
   pdl_wait_primary();
   const int cap = p.table_stride * kBlockTokens;
+  const int moves = ws.moves[0];
+  // Rows read remap while moving blocks' entries go from a place in the list to the id it stands for:
+  // either says the same.
+  for (int r = blockIdx.x * kCopyThreads + threadIdx.x; r < moves; r += gridDim.x * kCopyThreads) {
+    const int to = ws.list[r], from = ws.list[moves + r];
+    out.remap[from] = to;
+    out.ref_counts[to] = p.ref_counts[from];
+  }
   for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
     int len = p.seq_lens[row];
     if (len < 0 || len > cap) {
@@ -340,14 +374,14 @@ __global__ void __launch_bounds__(kCopyThreads) compact_apply_kernel(const PoolP
     for (int j = threadIdx.x; j < p.table_stride; j += kCopyThreads) {
       int id = p.tables[base + j];
       if (j < nb) {
-        const int to = valid_id(id, p.num_blocks) ? out.remap[id] : -1;
+        int to = valid_id(id, p.num_blocks) ? out.remap[id] : -1;
+        if (to < -1) to = ws.list[-2 - to - moves];
         if (to >= 0) id = to;
         else report(AEG_DEVERR_BLOCK_ID_RANGE);
       }
       out.tables[base + j] = id;
     }
   }
-  const int moves = ws.moves[0];
   const int64_t items = moves * p.segs;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int64_t r = item / p.segs;
@@ -493,7 +527,7 @@ int aeg_compact_blocks(void* pool, size_t block_bytes, int64_t num_blocks, const
   aeg::CompactOut out{block_tables_out, ref_counts_out, remap, num_live};
   AEG_CHECK_CUDA(aeg::launch(aeg::compact_plan_kernel, 1, aeg::kPlanThreads, s, p, ws, out));
   // At most half of the blocks move: free ones below the number of live ones, one for each live one beyond.
-  const int64_t work = std::max<int64_t>(num_blocks / 2 * p.segs, rows);
+  const int64_t work = std::max<int64_t>(num_blocks / 2 * std::max<int64_t>(p.segs, 1), rows);
   const int64_t grid = std::max<int64_t>(std::min<int64_t>(work, int64_t(aeg::num_sms()) * 8), 1);
   AEG_CHECK_CUDA(aeg::launch(aeg::vectors(p) ? aeg::compact_apply_kernel<true> : aeg::compact_apply_kernel<false>, grid,
                              aeg::kCopyThreads, s, p, ws, out));

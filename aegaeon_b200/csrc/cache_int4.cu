@@ -97,18 +97,7 @@ __global__ void __launch_bounds__(kThreads) write_int4_kernel(const Rows p) {
       if (h0 + i >= p.heads) break;
       uint2 q[kTokens];
 #pragma unroll
-      for (int j = 0; j < kTokens; ++j) {
-        float x[8];
-        const uint4& u = v[j * kHeads + i];
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const float2 f = unpack2<T>(w[n]);
-          x[2 * n] = f.x;
-          x[2 * n + 1] = f.y;
-        }
-        q[j] = int4_quantise<T>(x);
-      }
+      for (int j = 0; j < kTokens; ++j) q[j] = int4_quantise<T>(v[j * kHeads + i]);
 #pragma unroll
       for (int j = 0; j < kTokens; ++j) {
         if (slot[j] < 0) continue;

@@ -76,13 +76,39 @@ __device__ __forceinline__ float to_float<__half>(__half v) { return __half2floa
 template <>
 __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// A scale rounded as if from infinite precision, for an exact span: the quotient cut off at 24 bits with
-// a sticky last bit, then T's rounding.
+// A scale rounded as if from infinite precision, for an exact span well within fp32's range: the quotient
+// span / 15 by the rounded 1 / 15 and one correction is the nearest of 24 bits, the sign of its exact
+// remainder says on which side of it the true one lies, and rounding that to odd (cut off, with a sticky
+// last bit) leaves T's rounding as if made from the true quotient.
 template <typename T>
 __device__ __forceinline__ T scale_of_exact(float span) {
-  const float q = __fdiv_rz(span, 15.f);
-  const uint32_t sticky = fmaf(-15.f, q, span) != 0.f ? 1u : 0u;
-  return from_float<T>(__uint_as_float(__float_as_uint(q) | sticky));
+  constexpr float kFifteenth = 1.f / 15.f;
+  const float q0 = span * kFifteenth;
+  const float q = fmaf(fmaf(-15.f, q0, span), kFifteenth, q0);
+  const float rest = fmaf(-15.f, q, span);
+  uint32_t bits = __float_as_uint(q) - (rest < 0.f ? 1u : 0u);
+  if (rest != 0.f) bits |= 1u;
+  return from_float<T>(__uint_as_float(bits));
+}
+
+// 1 / s rounded to nearest, for a value s of T: one Newton step from the approximate reciprocal. With 8 or 11
+// significant bits in s that is the rounded one from any start within 2 ulp (tried for every mantissa).
+__device__ __forceinline__ float reciprocal_of_t(float s) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return fmaf(r, fmaf(-s, r, 1.f), r);
+}
+
+// A lane's 8 elements.
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& raw, float (&x)[8]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const float2 f = unpack2<T>(w[n]);
+    x[2 * n] = f.x;
+    x[2 * n + 1] = f.y;
+  }
 }
 
 __device__ __forceinline__ uint32_t pair_of(uint32_t scale, uint32_t lo) { return scale | (lo << 16); }
@@ -92,7 +118,9 @@ __device__ __forceinline__ uint32_t pair_of(uint32_t scale, uint32_t lo) { retur
 // |d - c s| <= s and d <= 16 s or so. Only where it is exactly half a scale does the rounding error e of
 // d = x - minimum itself count.
 template <typename T>
-__device__ __noinline__ uint2 int4_quantise_any(const float (&x)[8], float lo, float hi) {
+__device__ __noinline__ uint2 int4_quantise_any(uint4 raw, float lo, float hi) {
+  float x[8];
+  unpack8<T>(raw, x);
   const bool ok = isfinite(hi - lo);
   const T scale = round_once<T>(ok ? (static_cast<double>(hi) - static_cast<double>(lo)) / 15.0 : 0.0);
   float s = to_float<T>(scale);
@@ -132,10 +160,12 @@ __device__ __noinline__ uint2 int4_quantise_any(const float (&x)[8], float lo, f
 // or without a finite span take the general form, with their warp. Writing a prompt batch of 11,348
 // tokens x 4 heads took 21.7 us with the general form alone.
 template <typename T>
-__device__ __forceinline__ uint2 int4_quantise(const float (&x)[8]) {
+__device__ __forceinline__ uint2 int4_quantise(const uint4& raw) {
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr float kLeast = kHalf ? 0x1p-12f : 0x1p-15f;
   constexpr float kNormal = kHalf ? 0x1p-14f : 1e-30f;  // least scale of the short form
+  float x[8];
+  unpack8<T>(raw, x);
   float lo = x[0], hi = x[0], least = fabsf(x[0]);
 #pragma unroll
   for (int n = 1; n < 8; ++n) {
@@ -151,9 +181,9 @@ __device__ __forceinline__ uint2 int4_quantise(const float (&x)[8]) {
   }
   const float span = hi - lo;
   const bool sure = (least > span * kLeast || (kHalf && span < 0.5f)) && span > 16.f * kNormal && span < 3e38f;
-  if (!__all_sync(0xffffffffu, sure)) return int4_quantise_any<T>(x, lo, hi);
+  if (!__all_sync(0xffffffffu, sure)) return int4_quantise_any<T>(raw, lo, hi);
   const T scale = scale_of_exact<T>(span);
-  const float s = to_float<T>(scale), r = __frcp_rn(s);
+  const float s = to_float<T>(scale), r = reciprocal_of_t(s);
   uint32_t word = 0;
 #pragma unroll
   for (int n = 0; n < 8; ++n) {

@@ -55,7 +55,7 @@ def test_write_changes_the_named_rows_alone(cuda_device, dtype, T, Hkv):
 
 @BOTH
 def test_ties_subnormals_offsets_and_wide_spreads(cuda_device, dtype):
-    rows = _hard_rows(dtype, 400, torch.Generator().manual_seed(11))
+    rows = _hard_rows(dtype, 6000, torch.Generator().manual_seed(11))
     n = rows.size(0) // 2 * 2
     x = rows[:n].view(-1, 1, 128)
     T = x.size(0)
