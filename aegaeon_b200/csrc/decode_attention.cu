@@ -657,7 +657,10 @@ __device__ __forceinline__ float4 ld_cg_f4(const float4* ptr) {
 //     g, g + 4, g + 8, g + 12 and the 4 groups are combined by xor shuffles.
 // Either way a lane folds at most 4 pieces, whose 16 row loads share one round trip.
 
-template <typename T, typename WriteRow>
+// With kJoint a lane's pieces are weighted by one maximum of the batch (their exponentials do not wait
+// for one another) instead of being folded in one by one.
+
+template <typename T, bool kJoint, typename WriteRow>
 __device__ __forceinline__ void merge_small(const AttnParams& p, const int4& e, int item, int lane, bool by_pieces,
                                             WriteRow& write_row) {
   constexpr int kLanes = 32 / kMergeLaneGroups;  // lanes per group
@@ -689,6 +692,31 @@ __device__ __forceinline__ void merge_small(const AttnParams& p, const int4& e, 
       if (i >= cnt) break;
 #pragma unroll
       for (int k = 0; k < kCols; ++k) after_loads(ml[i], v[i][k]);
+    }
+    if constexpr (kJoint) {
+      float Mn = M;
+#pragma unroll
+      for (int i = 0; i < kMergeHeadBatch; ++i)
+        if (i < cnt) Mn = fmaxf(Mn, ml[i].x);
+      const float r = M != -INFINITY ? ex2(M - Mn) : 0.f;
+#pragma unroll
+      for (int k = 0; k < kCols; ++k) acc[k] = make_float4(acc[k].x * r, acc[k].y * r, acc[k].z * r, acc[k].w * r);
+      L *= r;
+#pragma unroll
+      for (int i = 0; i < kMergeHeadBatch; ++i) {
+        if (i >= cnt) break;
+        const float w = ex2(ml[i].x - Mn);
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) {
+          acc[k].x = fmaf(w, v[i][k].x, acc[k].x);
+          acc[k].y = fmaf(w, v[i][k].y, acc[k].y);
+          acc[k].z = fmaf(w, v[i][k].z, acc[k].z);
+          acc[k].w = fmaf(w, v[i][k].w, acc[k].w);
+        }
+        L = fmaf(w, ml[i].y, L);
+      }
+      M = Mn;
+      continue;
     }
 #pragma unroll
     for (int i = 0; i < kMergeHeadBatch; ++i) {
@@ -748,7 +776,7 @@ __device__ __forceinline__ void merge_small(const AttnParams& p, const int4& e, 
 //   * q > 1 (more than kMergeBatch pieces): the item is (head item / q, dimension chunk
 //     item % q); lane = (piece group g, float4 column c) with 32 / q columns per chunk, group g
 //     takes pieces g, g + q, ..., and the q groups are combined by xor shuffles.
-template <typename T, int kLoads = kMergeBatch>
+template <typename T, int kLoads = kMergeBatch, bool kJoint = false>
 __device__ __forceinline__ void merge_item(const AttnParams& p, const int4& e, int item, int lane) {
   const int G = p.G;
   const int shape = e.z >> 16, q = shape & 0xff, hg = shape >> 8, ns = e.z & 0xffff;
@@ -782,7 +810,7 @@ __device__ __forceinline__ void merge_item(const AttnParams& p, const int4& e, i
   };
 
   if (q == 1) {
-    merge_small<T>(p, e, item, lane, hg == 1, write_row);
+    merge_small<T, kJoint>(p, e, item, lane, hg == 1, write_row);
     return;
   }
 
@@ -809,10 +837,31 @@ __device__ __forceinline__ void merge_item(const AttnParams& p, const int4& e, i
       if (i >= cnt) break;
       after_loads(ml[i], v[i]);
     }
+    if constexpr (kJoint) {
+      float Mn = M;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      if (i >= cnt) break;
-      fold(M, L, acc, ml[i], v[i]);
+      for (int i = 0; i < kLoads; ++i)
+        if (i < cnt) Mn = fmaxf(Mn, ml[i].x);
+      const float r = M != -INFINITY ? ex2(M - Mn) : 0.f;
+      acc = make_float4(acc.x * r, acc.y * r, acc.z * r, acc.w * r);
+      L *= r;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        if (i >= cnt) break;
+        const float w = ex2(ml[i].x - Mn);
+        acc.x = fmaf(w, v[i].x, acc.x);
+        acc.y = fmaf(w, v[i].y, acc.y);
+        acc.z = fmaf(w, v[i].z, acc.z);
+        acc.w = fmaf(w, v[i].w, acc.w);
+        L = fmaf(w, ml[i].y, L);
+      }
+      M = Mn;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        if (i >= cnt) break;
+        fold(M, L, acc, ml[i], v[i]);
+      }
     }
   }
   for (int off = 1 << lc; off < 32; off <<= 1) {

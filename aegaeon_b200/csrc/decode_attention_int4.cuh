@@ -776,6 +776,8 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
       }
       if (ready_entry != entry) {
         const int w0 = me.w & 0xffff, nw = me.w >> 16;
+        // 32 flags at a time (asking for all of a long pair's 200 in one round trip, with a fence behind it,
+        // took 4 us longer: the polls of hundreds of warps delay the stamps themselves).
         int ok = 1;
         for (int i = 0; i < nw && ok; i += 32) {
           const int ww = w0 + i + lane;
@@ -789,7 +791,7 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
         }
         ready_entry = entry;
       }
-      merge_item<T, SL::kMergeLoads>(p, me, k, lane);
+      merge_item<T, SL::kMergeLoads, true>(p, me, k, lane);
       ++k;
     }
   } else if (lane == 0) {
