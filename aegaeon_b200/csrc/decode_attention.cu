@@ -7,8 +7,8 @@
 // KV head h / (Hq / Hkv).
 //
 // Design (memory-bound: every K/V byte is read exactly once per layer call):
-//   * Work item = one 16-token block of one (sequence b, KV head h) pair. A plan kernel, run
-//     once per decode step, cuts the batch's items (in pair order) into W contiguous ranges of
+//   * Work item = one 16-token block of one (sequence b, KV head h) pair. A plan, made once per
+//     decode step (scans in one CTA, lists written by the whole GPU), cuts the batch's items (in pair order) into W contiguous ranges of
 //     equal size, one per worker warp of the attention grid (W = 8 warps x one CTA per SM).
 //     A worker's range is a list of units (pieces of pairs); a pair cut by a worker start is
 //     "split", and its units write partials. A unit record carries the pair, its block range,

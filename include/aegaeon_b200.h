@@ -16,6 +16,11 @@
  *   aeg_prefill_attention  vLLM 0.5.1 FlashAttention backend prompt call `flash_attn_varlen_func`
  *   aeg_prepare_step_inputs the per-step Python loops of Worker._prepare_model_inputs
  *                          (worker.py:596-682), on the device
+ *   aeg_*_int4             no counterpart: the cache write, read-back and decode attention of a KV
+ *                          cache held in 4 bits
+ *   aeg_rotary_multi_axis  the model's rotary embedding, with positions on several axes
+ *   aeg_fork_blocks,       no counterpart: blocks shared between requests (the reference gives every
+ *   aeg_free/compact_...   request blocks of its own, aegaeon/aegaeon/block_manager.py)
  *   aeg_decode_plan +      vLLM 0.5.1 FlashAttention backend decode call
  *   aeg_paged_attn_decode  `flash_attn_with_kvcache(q, K_l, V_l, block_table, cache_seqlens, ...)`
  *                          with the metadata built at aegaeon/aegaeon/worker.py:554-713
