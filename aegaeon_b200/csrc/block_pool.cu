@@ -235,8 +235,8 @@ __global__ void __launch_bounds__(kCopyThreads) fork_apply_kernel(const PoolPara
     for (int j = threadIdx.x; j < nb; j += kCopyThreads) {
       const int id = (j == nb - 1 && e.w >= 0) ? e.w : from[j];
       to[j] = id;
-      if (valid_id(id, p.num_blocks)) atomicAdd(&p.ref_counts[id], 1);
-      else report(AEG_DEVERR_BLOCK_ID_RANGE);
+      if (!valid_id(id, p.num_blocks)) report(AEG_DEVERR_BLOCK_ID_RANGE);
+      else if (atomicAdd(&p.ref_counts[id], 1) <= 0 && id != e.w) report(AEG_DEVERR_POOL_ENTRY);  // a free block in a row
     }
   }
   const int64_t items = n * p.segs;

@@ -1873,6 +1873,7 @@ int decode_int4(void* out, int64_t out_stride, const void* q, int64_t q_stride, 
   AEG_CHECK_ARG(aligned(q, 4) && q_stride % 2 == 0, "decode_int4: q must be 4-byte aligned with an even token stride");
   AEG_CHECK_ARG(aligned(out, 2), "decode_int4: out must be 2-byte aligned");
   AEG_CHECK_ARG(aligned(block_tables, 4) && aligned(seq_lens, 4), "decode_int4: int32 arrays must be aligned");
+  AEG_CHECK_ARG(std::isfinite(scale), "decode_int4: the scale is not finite");
   AEG_CHECK_ARG((flags & ~AEG_DECODE_PREFETCH) == 0, "decode_int4: flags 0x%x, only AEG_DECODE_PREFETCH is known", flags);
   const bool one = Hq / Hkv <= 8, bf = dtype == AEG_DTYPE_BF16;
   st = bf ? (one ? check_attn_int4<__nv_bfloat16, 1>(L.max_warps) : check_attn_int4<__nv_bfloat16, 2>(L.max_warps))

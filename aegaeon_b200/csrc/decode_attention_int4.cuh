@@ -92,6 +92,8 @@ constexpr float kMiddle = 8.f;
 template <typename T>
 constexpr uint32_t kScaleInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
 template <typename T>
+constexpr float kScaleLeast = std::is_same<T, __half>::value ? 0x1p-14f : 0x1p-100f;  // smaller ones count as this
+template <typename T>
 constexpr uint32_t kScaleMantissa = std::is_same<T, __half>::value ? 0x3ffu : 0x7fu;
 constexpr float kValueMiddle = 8.f;
 
@@ -592,7 +594,7 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
       if (top > vlim && top < kScaleInf<T>) {
         // The power of two above the scale, kept in range for the tiniest ones. NaN needs no room: it
         // makes the result NaN by itself.
-        const float t = fmaxf(unpack2<T>(top).x, 6.103515625e-05f);
+        const float t = fmaxf(unpack2<T>(top).x, kScaleLeast<T>);
         const uint32_t e = __float_as_uint(t) >> 23;  // t in [2^(e - 127), 2^(e - 126))
         const float next = __uint_as_float((253u - e) << 23) * kTop;
         grow = vlim == 0 ? 1.f : next / vmul;  // nothing but zeros was added before the first scale

@@ -829,7 +829,8 @@ def compact_blocks(kv_cache: torch.Tensor, ref_counts: torch.Tensor, block_table
     The live blocks' contents are copied within ``kv_cache``: the k-th live id that is not below the
     number of live blocks goes to the k-th free id below it. ``ref_counts``, ``block_tables`` and
     ``seq_lens`` are only read: adopt the returned tables and counts. The old places keep their
-    contents, so a step in flight on the old tables stays right until their ids are given out.
+    contents, so reads through the old tables stay right until their ids are given out; writes through
+    them after this call do not reach the moved blocks.
     """
     index, N, width, rows = _check_shared(ref_counts, block_tables, seq_lens)
     nbytes = _check_pool(kv_cache, index, N)

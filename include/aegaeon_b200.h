@@ -398,7 +398,7 @@ AEG_API int aeg_gather_cache_int4(void* key, void* value, int64_t key_stride, in
  * NaN). The workspace is planned by aeg_decode_plan_int4 (same size and arguments as aeg_decode_plan;
  * a plan of the other kind raises AEG_DEVERR_PLAN_MISMATCH). A block id outside the pool raises
  * AEG_DEVERR_BLOCK_ID_RANGE and its tokens are left out. flags: 0 or AEG_DECODE_PREFETCH. D = 128,
- * Hq / Hkv <= 16, `kv_cache` 16-byte aligned. */
+ * Hq / Hkv <= 16, `kv_cache` 16-byte aligned, `scale` finite. */
 AEG_API int aeg_decode_plan_int4(void* workspace, size_t workspace_bytes, const int32_t* block_tables,
                                  int table_stride, const int32_t* seq_lens, int B, int Hq, int Hkv,
                                  int D, void* stream);
@@ -444,7 +444,8 @@ AEG_API int aeg_rotary_multi_axis(void* q_out, int64_t q_out_stride, void* k_out
  * is outside the table, the source's length is outside it, the target row is not empty or an earlier
  * entry names it; AEG_DEVERR_BLOCK_ID_RANGE instead when the block to copy is outside the pool, and
  * AEG_DEVERR_POOL_EMPTY when no free block is left (later entries that need none still proceed).
- * Sources are read as they were before the call. */
+ * Sources are read as they were before the call; their blocks must be live (sharing a free one raises
+ * AEG_DEVERR_POOL_ENTRY, and the call may have given it out). */
 AEG_API size_t aeg_fork_blocks_workspace_size(int64_t n);
 AEG_API int aeg_fork_blocks(void* pool, size_t block_bytes, int64_t num_blocks, int32_t* ref_counts,
                             int32_t* block_tables, int table_stride, int rows, int32_t* seq_lens,
@@ -463,8 +464,9 @@ AEG_API int aeg_free_blocks(int64_t num_blocks, int32_t* ref_counts, const int32
 /* aeg_compact_blocks: moves the live blocks (ref_counts > 0) to the ids below their number: the k-th
  * live id from num_live on goes to the k-th free id below it, the others stay. Writes the new tables
  * and counts, remap[old id] = new id (-1 for a free block) and *num_live; the inputs keep their
- * values, and so do the moved blocks' old places, so that work in flight on the old tables stays
- * right until those ids are given out again. block_tables_out may be block_tables. A table entry in
+ * values, and so do the moved blocks' old places, so that reads through the old tables stay right
+ * until those ids are given out again (writes through them no longer reach the moved blocks).
+ * block_tables_out may be block_tables. A table entry in
  * use that is outside the pool or free is left as it is (AEG_DEVERR_BLOCK_ID_RANGE); a length outside
  * the table is clamped (AEG_DEVERR_SEQ_LEN_RANGE). Pointers of outputs are DEVICE memory. */
 AEG_API size_t aeg_compact_blocks_workspace_size(int64_t num_blocks);

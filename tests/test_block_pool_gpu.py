@@ -137,6 +137,16 @@ def test_ids_outside_the_pool_are_reported(cuda_device):
     b.free([0, 2])
 
 
+def test_sharing_a_free_block_is_reported(cuda_device):
+    b = Both(cuda_device, 8, 4, 2)
+    b.fill([0], [32])
+    b.o.counts[b.o.tables[0][0]] = 0
+    b.sync_in()
+    ops.fork_blocks(b.kv, b.counts, b.tables, b.lens, [0], [1])
+    b.o.fork([0], [1])
+    b.check(("entry",))
+
+
 def test_more_forks_than_one_pass_over_the_entries(cuda_device):
     R = 2600
     b = Both(cuda_device, 4000, R, 2, (3,))

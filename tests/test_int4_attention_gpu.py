@@ -119,6 +119,22 @@ def test_scales_of_every_size(cuda_device, dtype, kind):
     _check(cuda_device, _q(dtype, 4, 8), _cache(dtype, 60, 1, 2, 8, kind), 0, make_tables(lens, 60, 1), lens)
 
 
+@pytest.mark.parametrize("size", [1e-25, 1e-12, 1e8, 1e30])
+def test_bf16_values_far_from_one(cuda_device, size):
+    """Value scales of every size bf16 has, over 2^10 within a sequence."""
+    dtype, lens = torch.bfloat16, [300, 20, 7]
+    cache = _cache(dtype, 30, 1, 2, 8)
+    g = torch.Generator().manual_seed(int(-math.log10(size)) % 97)
+    s = size * torch.pow(2.0, -10 * torch.rand(30, 1, 2, 16, 2, generator=g))
+    pairs = cache[..., 1088:].view(30, 1, 2, 16, 2, 2)
+    pairs[..., 0] = s.to(dtype)
+    pairs[..., 1] = (-7 * s + size * 0.1 * torch.randn(s.shape, generator=g)).to(dtype)
+    q, tables = _q(dtype, 3, 8), make_tables(lens, 30, 1)
+    got = _run(cuda_device, q, cache, 0, tables, lens)
+    want = ref.attention(q, cache, 0, tables, lens, SCALE)
+    assert ((got.double() - want).abs() <= _bound(want, q, cache, 0, tables, lens, SCALE)).all()
+
+
 @BOTH
 def test_long_sequences_split_over_many_warps(cuda_device, dtype):
     lens = [20000, 7, 9001]
@@ -294,7 +310,7 @@ def test_refusals_and_empty_batch(cuda_device):
     ops.paged_attention_decode_int4(**good)
     for bad in (dict(query=q.bfloat16()), dict(query=q[:, :3], out=good["out"][:, :3]), dict(kv_cache=cache.bfloat16()), dict(layer=1),
                 dict(layer=-1), dict(seq_lens=sl.long()), dict(block_tables=tables[:1]), dict(out=good["out"][:, :2]), dict(out=q.float()),
-                dict(block_tables=tables[:, :0]), dict(kv_cache=cache[:, :, :, :1151]), dict(query=q.cpu()), dict(seq_lens=sl.cpu()),
+                dict(block_tables=tables[:, :0]), dict(scale=float("nan")), dict(scale=float("inf")), dict(kv_cache=cache[:, :, :, :1151]), dict(query=q.cpu()), dict(seq_lens=sl.cpu()),
                 dict(query=torch.empty(2, 34, 128, dtype=torch.float16, device=cuda_device), out=torch.empty(2, 34, 128, dtype=torch.float16, device=cuda_device))):
         with pytest.raises((ValueError, NotImplementedError)):
             ops.paged_attention_decode_int4(**dict(good, **bad))
