@@ -34,12 +34,13 @@ def _stream(device: torch.device) -> ctypes.c_void_p:
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _launch(index: int, what: str, fn, *args) -> None:
     """Calls ``fn(*args, stream)`` with device ``index`` current, on its current stream. A decode step is
     dozens of such calls: the device is switched only when it has to be."""
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         st = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -53,6 +54,12 @@ def _on_device(index: int, t: torch.Tensor, name: str) -> None:
     if not isinstance(t, torch.Tensor) or t.get_device() != index:
         _require_cuda(t, name)
         raise ValueError(f"{name} is on {t.device}, the operation runs on cuda:{index}")
+
+
+def _on_devices(index: int, tensors: dict) -> None:
+    """Raises the error of the tensor that is not on device ``index`` (after a comparison found one)."""
+    for name, t in tensors.items():
+        _on_device(index, t, name)
 
 
 def _token_rows(t: torch.Tensor, name: str, what: str) -> torch.Size:
@@ -608,9 +615,8 @@ def _int4_move(fn, what: str, key: torch.Tensor, value: torch.Tensor, kv_cache: 
         raise ValueError("slot_mapping must be int64 [T]")
     slot_mapping = slot_mapping.contiguous()
     index = kv_cache.get_device()
-    _on_device(index, key, "key")
-    _on_device(index, value, "value")
-    _on_device(index, slot_mapping, "slot_mapping")
+    if not (index == key.get_device() == value.get_device() == slot_mapping.get_device()):
+        _on_devices(index, dict(key=key, value=value, slot_mapping=slot_mapping))
     _launch(index, what, fn, key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0), base, block_stride, N,
             slot_mapping.data_ptr(), T, Hkv, D, _DTYPES[dtype])
 
@@ -640,9 +646,7 @@ def gather_cache_int4(kv_cache: torch.Tensor, layer: int, slot_mapping: torch.Te
         _require_cuda(slot_mapping, "slot_mapping")
         if kv_cache.dim() != 4:
             raise ValueError(f"kv_cache must be a 4-bit cache (N, L, Hkv, {INT4_TILE})")
-        shape = (slot_mapping.numel(), kv_cache.size(2), 128)
-        key = torch.empty(shape, dtype=kv_cache.dtype, device=kv_cache.device)
-        value = torch.empty_like(key)
+        key, value = kv_cache.new_empty((2, slot_mapping.numel(), kv_cache.size(2), 128)).unbind()
     _int4_move(lib.aeg_gather_cache_int4, "gather_cache_int4", key, value, kv_cache, layer, slot_mapping)
     return key, value
 
@@ -704,14 +708,14 @@ def rotary_multi_axis(query: torch.Tensor, key: torch.Tensor, positions: torch.T
         raise ValueError(f"inv_freq must be float32 [{half}], one per frequency of the sections")
     inv_freq = inv_freq.contiguous()
     index = query.get_device()
-    for name, t in (("key", key), ("positions", positions), ("inv_freq", inv_freq)):
-        _on_device(index, t, name)
+    if not (index == key.get_device() == positions.get_device() == inv_freq.get_device()):
+        _on_devices(index, dict(key=key, positions=positions, inv_freq=inv_freq))
     if query_out is None:
-        query_out = torch.empty_like(query, memory_format=torch.contiguous_format)
+        query_out = torch.empty_like(query) if query.is_contiguous() else query.new_empty(query.shape)
     else:
         _check_rotary_out(index, query_out, query, "query_out")
     if key_out is None:
-        key_out = torch.empty_like(key, memory_format=torch.contiguous_format)
+        key_out = torch.empty_like(key) if key.is_contiguous() else key.new_empty(k_shape)
     else:
         _check_rotary_out(index, key_out, key, "key_out")
     _launch(index, "rotary_multi_axis", lib.aeg_rotary_multi_axis, query_out.data_ptr(), query_out.stride(0),
@@ -792,7 +796,7 @@ def fork_blocks(kv_cache: torch.Tensor, ref_counts: torch.Tensor, block_tables: 
     # One allocation: the result, then the entries' scratch (16-byte aligned).
     ws_bytes = lib.aeg_fork_blocks_workspace_size(n)
     at = (n + 3) // 4 * 4
-    buf = torch.empty(at + (ws_bytes + 3) // 4, dtype=torch.int32, device=ref_counts.device)
+    buf = ref_counts.new_empty(at + (ws_bytes + 3) // 4)
     new_blocks = buf[:n]
     if n == 0:
         return new_blocks
@@ -835,11 +839,12 @@ def compact_blocks(kv_cache: torch.Tensor, ref_counts: torch.Tensor, block_table
     index, N, width, rows = _check_shared(ref_counts, block_tables, seq_lens)
     nbytes = _check_pool(kv_cache, index, N)
     out = CompactedBlocks(torch.empty_like(block_tables), torch.empty_like(ref_counts), torch.empty_like(ref_counts),
-                          torch.empty(1, dtype=torch.int32, device=ref_counts.device))
-    ws = torch.empty(lib.aeg_compact_blocks_workspace_size(N), dtype=torch.uint8, device=ref_counts.device)
+                          ref_counts.new_empty(1))
+    ws_bytes = lib.aeg_compact_blocks_workspace_size(N)
+    ws = ref_counts.new_empty((ws_bytes + 3) // 4)
     _launch(index, "compact_blocks", lib.aeg_compact_blocks, kv_cache.data_ptr(), nbytes, N, ref_counts.data_ptr(),
             block_tables.data_ptr(), width, rows, seq_lens.data_ptr(), out.ref_counts.data_ptr(),
-            out.block_tables.data_ptr(), out.remap.data_ptr(), out.num_live.data_ptr(), ws.data_ptr(), ws.size(0))
+            out.block_tables.data_ptr(), out.remap.data_ptr(), out.num_live.data_ptr(), ws.data_ptr(), ws_bytes)
     return out
 
 
@@ -1096,10 +1101,8 @@ def paged_attention_decode_int4(out: torch.Tensor, query: torch.Tensor, kv_cache
     if _token_rows(out, "out", "query's shape") != shape or out.dtype != dtype:
         raise ValueError("out must match query's shape and dtype")
     index = query.get_device()
-    _on_device(index, kv_cache, "kv_cache")
-    _on_device(index, block_tables, "block_tables")
-    _on_device(index, seq_lens, "seq_lens")
-    _on_device(index, out, "out")
+    if not (index == kv_cache.get_device() == block_tables.get_device() == seq_lens.get_device() == out.get_device()):
+        _on_devices(index, dict(kv_cache=kv_cache, block_tables=block_tables, seq_lens=seq_lens, out=out))
     if B == 0:
         return
     if block_tables.size(1) == 0:
@@ -1109,7 +1112,8 @@ def paged_attention_decode_int4(out: torch.Tensor, query: torch.Tensor, kv_cache
     elif not plan.matches(B, Hq, Hkv, D, block_tables, seq_lens, "int4"):
         raise ValueError("plan was built for a different batch / head layout / block tables / sequence lengths / cache")
     ws = plan.workspace
-    _on_device(index, ws, "plan workspace")
+    if ws.get_device() != index:
+        _on_device(index, ws, "plan workspace")
     _launch(index, "paged_attention_decode_int4", lib.aeg_paged_attn_decode_int4, out.data_ptr(), out.stride(0),
             query.data_ptr(), query.stride(0), base, block_stride, N, block_tables.data_ptr(), block_tables.stride(0),
             seq_lens.data_ptr(), B, Hq, Hkv, D, float(scale), _DTYPES[dtype], ws.data_ptr(), ws.numel(),
