@@ -69,6 +69,7 @@ constexpr int kBlockTokens = 16;
 constexpr int kMaxWarps = 4096;         // worker warps of one launch the workspace is sized for
 constexpr int kPlanThreads = 256;
 constexpr int kUnitCost = 2;           // plan cost of starting a pair, in blocks (query load, epilogue)
+constexpr int kUnitCostInt4 = 4;       // the same over a 4-bit cache (64 sequences 10.3 us a layer, 11.0 at 2)
 constexpr int kPlanLongUnits = 4;       // a pair with more units has them written by the whole plan CTA
 constexpr int kPlanLongPairs = 512;     // capacity of the plan's list of such pairs
 constexpr int kPlanCachedSeqs = 4096;   // sequences whose block counts the plan keeps in smem
@@ -166,7 +167,7 @@ inline WsPtrs ws_ptrs(void* ws, const WsLayout& L) {
 
 // ---------------------------------------------------------------------------------------
 // Plan kernel (one CTA). The (pair, block) items of the batch, in pair order, each non-empty
-// pair preceded by kUnitCost virtual items (the cost of starting a pair), form a cost axis of
+// pair preceded by unit_cost virtual items (the cost of starting a pair), form a cost axis of
 // I positions, cut into Wp = min(W, I) contiguous ranges of equal size (up to one position),
 // one per worker warp: worker w < Wp starts at position floor(w * I / Wp), workers from Wp on
 // get nothing. Units are the pieces of pairs' blocks between pair ends and worker starts; a
@@ -290,7 +291,7 @@ static_assert(sizeof(PlanScan) == 32 && sizeof(PlanPair) == 32, "16-byte aligned
 template <bool kScan>
 __global__ void __launch_bounds__(kPlanThreads, 1)
 decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tables, int B, int Hkv,
-                   int G, int table_stride, int W, WsPtrs ws, PlanScan* scan) {
+                   int G, int table_stride, int W, int unit_cost, WsPtrs ws, PlanScan* scan) {
   __shared__ long long s_red[kPlanThreads / 32];
   __shared__ int s_warp[kPlanThreads / 32];
   __shared__ int s_nb[kPlanCachedSeqs];  // blocks per sequence (first kPlanCachedSeqs sequences)
@@ -317,7 +318,7 @@ decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tab
   long long local = 0;
   for (int p = p0; p < p1; ++p) {
     const int nb = blocks_of(p / Hkv);
-    local += nb > 0 ? nb + kUnitCost : 0;
+    local += nb > 0 ? nb + unit_cost : 0;
   }
   long long I = 0;
   const long long o_t = block_excl_scan64(local, s_red, I);
@@ -351,14 +352,14 @@ decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tab
       n_mi += merge_items(merge_shape(0, G), G);
       continue;
     }
-    const int c = cuts(o + kUnitCost, nb);
+    const int c = cuts(o + unit_cost, nb);
     n_units += c + 1;
     if (c > 0) {
       ++n_sp;
       n_slots += c + 1;
       n_mi += merge_items(merge_shape(c + 1, G), G);
     }
-    o += nb + kUnitCost;
+    o += nb + unit_cost;
   }
   int U = 0, S = 0, SL = 0;
   int u = block_excl_scan(n_units, s_warp, U);
@@ -393,7 +394,7 @@ decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tab
     for (int p = p0; p < p1; ++p) {
       const int nb = blocks_of(p / Hkv);
       pairs[p] = PlanPair{o, mo, u, sp, slot, 0};
-      const int c = nb > 0 ? cuts(o + kUnitCost, nb) : 0;
+      const int c = nb > 0 ? cuts(o + unit_cost, nb) : 0;
       if (nb == 0 || c > 0) {
         ++sp;
         mo += merge_items(merge_shape(nb == 0 ? 0 : c + 1, G), G);
@@ -401,7 +402,7 @@ decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tab
       if (nb > 0) {
         u += c + 1;
         if (c > 0) slot += c + 1;
-        o += nb + kUnitCost;
+        o += nb + unit_cost;
       }
     }
     return;
@@ -429,7 +430,7 @@ decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tab
     ws.units[2 * u_idx] = ra;
     ws.units[2 * u_idx + 1] = rb;
     const long long w_hi = wk.le(xa);
-    for (long long w = wk.le((k == 0 ? o0 - kUnitCost : xa) - 1); w < w_hi; ++w) {
+    for (long long w = wk.le((k == 0 ? o0 - unit_cost : xa) - 1); w < w_hi; ++w) {
       ws.warp_rec[3 * w] = make_int4(u_idx, 0, 0, 0);
       ws.warp_rec[3 * w + 1] = ra;
       ws.warp_rec[3 * w + 2] = rb;
@@ -445,7 +446,7 @@ decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tab
       ws.split_pairs[sp++] = make_int4(p, 0, shape << 16, 0);
       continue;
     }
-    const long long ob = o + kUnitCost;  // position of the pair's first block
+    const long long ob = o + unit_cost;  // position of the pair's first block
     const int c = cuts(ob, nb);
     if (c > 0) {
       const int shape = merge_shape(c + 1, G), n_it = merge_items(shape, G);
@@ -500,7 +501,7 @@ decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tab
 constexpr int kListThreads = 64;
 __global__ void __launch_bounds__(kListThreads)
 plan_lists_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tables, int B, int Hkv, int G, int table_stride,
-                  int W, WsPtrs ws, const PlanScan* scan) {
+                  int W, int unit_cost, WsPtrs ws, const PlanScan* scan) {
   pdl_wait_primary();
   const int tid = threadIdx.x;
   const long long I = scan->items, MI = scan->merge_items;
@@ -521,7 +522,7 @@ plan_lists_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tabl
     const int b = p / Hkv;
     const int n_ctx = min(max(seq_lens[b], 0), cap);
     const int nb = (n_ctx + kBlockTokens - 1) / kBlockTokens;
-    const long long ob = r.o + kUnitCost;
+    const long long ob = r.o + unit_cost;
     const int c = nb > 0 ? static_cast<int>(wk.le(ob + nb - 1) - wk.le(ob)) : 0;
     if (nb == 0 || c > 0) {
       const int shape = merge_shape(nb == 0 ? 0 : c + 1, G), n_it = merge_items(shape, G);
@@ -1916,16 +1917,16 @@ int decode_int4(void* out, int64_t out_stride, const void* q, int64_t q_stride, 
 // Plans on `stream`: scans in one CTA, then the lists over the GPU where the pairs' records fit the
 // partial-result area; else (far more pairs than workers) all of it in one CTA.
 int launch_plan(const char* what, const int32_t* seq_lens, const int32_t* block_tables, int B, int Hkv, int G,
-                int table_stride, int W, void* workspace, const WsLayout& L, cudaStream_t stream) {
+                int table_stride, int W, int unit_cost, void* workspace, const WsLayout& L, cudaStream_t stream) {
   const WsPtrs ws = ws_ptrs(workspace, L);
   PlanScan* scan = reinterpret_cast<PlanScan*>(ws.part_ml);
   const int64_t P = int64_t(B) * Hkv;
   if (P == 0 || sizeof(PlanScan) + sizeof(PlanPair) * P > L.total - L.part_ml) {
-    decode_plan_kernel<false><<<1, kPlanThreads, 0, stream>>>(seq_lens, block_tables, B, Hkv, G, table_stride, W, ws, scan);
+    decode_plan_kernel<false><<<1, kPlanThreads, 0, stream>>>(seq_lens, block_tables, B, Hkv, G, table_stride, W, unit_cost, ws, scan);
     AEG_CHECK_LAUNCH(what);
     return AEG_OK;
   }
-  decode_plan_kernel<true><<<1, kPlanThreads, 0, stream>>>(seq_lens, block_tables, B, Hkv, G, table_stride, W, ws, scan);
+  decode_plan_kernel<true><<<1, kPlanThreads, 0, stream>>>(seq_lens, block_tables, B, Hkv, G, table_stride, W, unit_cost, ws, scan);
   AEG_CHECK_LAUNCH(what);
   cudaLaunchAttribute attr[1] = {pdl_attr()};
   cudaLaunchConfig_t cfg{};
@@ -1935,8 +1936,8 @@ int launch_plan(const char* what, const int32_t* seq_lens, const int32_t* block_
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   AEG_CHECK_CUDA(cudaLaunchKernelEx(&cfg, plan_lists_kernel, static_cast<const int*>(seq_lens),
-                                    static_cast<const int*>(block_tables), B, Hkv, G, table_stride, W, ws,
-                                    static_cast<const PlanScan*>(scan)));
+                                    static_cast<const int*>(block_tables), B, Hkv, G, table_stride, W, unit_cost,
+                                    ws, static_cast<const PlanScan*>(scan)));
   return AEG_OK;
 }
 
@@ -1952,7 +1953,8 @@ int plan_common(const char* what, void* workspace, size_t workspace_bytes, const
   const int W = int4 ? worker_warps_int4(Hq / Hkv) : worker_warps(Hq / Hkv);
   if (W > L.max_warps)
     return set_error(AEG_ERR_UNSUPPORTED, "%s: %d worker warps exceed the workspace's %d", what, W, L.max_warps);
-  const int launched = launch_plan(what, seq_lens, block_tables, B, Hkv, Hq / Hkv, table_stride, W, workspace, L,
+  const int launched = launch_plan(what, seq_lens, block_tables, B, Hkv, Hq / Hkv, table_stride, W,
+                                   int4 ? kUnitCostInt4 : kUnitCost, workspace, L,
                                    static_cast<cudaStream_t>(stream));
   if (launched != AEG_OK) return launched;
   mark_plan_fresh(workspace);
@@ -2116,7 +2118,8 @@ int aeg_paged_attn_decode_noalloc(void* out, int64_t out_stride, const void* q, 
   bool waited = false;
   st = order.enter(s, &waited);
   if (st != AEG_OK) return st;
-  st = aeg::launch_plan("decode_plan (noalloc)", seq_lens, block_tables, B, Hkv, Hq / Hkv, table_stride, W, scratch, L, s);
+  st = aeg::launch_plan("decode_plan (noalloc)", seq_lens, block_tables, B, Hkv, Hq / Hkv, table_stride, W, aeg::kUnitCost,
+                        scratch, L, s);
   if (st != AEG_OK) return st;
   dl.prm.plan_ready = 0;  // the plan kernel directly precedes this launch: read it after the wait
   return aeg::decode_launch(dl, s, order);

@@ -908,7 +908,7 @@ class DecodePlan:
 
     def stats(self) -> dict:
         """What the last ``plan`` built, read back from the workspace header (waits for the plan):
-        the cost-axis positions (blocks plus kUnitCost per non-empty (sequence, head) pair), the
+        the cost-axis positions (blocks plus the starting cost per non-empty (sequence, head) pair), the
         worker warps the positions were cut for, the units (pieces of pairs between pair ends and
         warp starts), the split-pair entries (pairs cut across warps, plus empty pairs), the
         partial-result slots those pieces write, and the split-merge items."""
