@@ -291,7 +291,7 @@ static_assert(sizeof(PlanScan) == 32 && sizeof(PlanPair) == 32, "16-byte aligned
 template <bool kScan>
 __global__ void __launch_bounds__(kPlanThreads, 1)
 decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tables, int B, int Hkv,
-                   int G, int table_stride, int W, int unit_cost, WsPtrs ws, PlanScan* scan) {
+                   int G, int table_stride, int W, int flags, int unit_cost, WsPtrs ws, PlanScan* scan) {
   __shared__ long long s_red[kPlanThreads / 32];
   __shared__ int s_warp[kPlanThreads / 32];
   __shared__ int s_nb[kPlanCachedSeqs];  // blocks per sequence (first kPlanCachedSeqs sequences)
@@ -332,7 +332,7 @@ decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tab
     }
     for (int w = tid; w <= W; w += kPlanThreads) ws.warp_rec[3 * w] = make_int4(0, 0, 0, 0);
     for (int w = tid; w < W; w += kPlanThreads) ws.merge_rec[w] = make_int4(0, 0, 0, 0);
-    for (int c = tid; c < W; c += kPlanThreads) ws.warp_flag[c * kFlagStride] = 0;
+    for (int c = tid; c < flags; c += kPlanThreads) ws.warp_flag[c * kFlagStride] = 0;
     return;
   }
   const int Wp = I < W ? static_cast<int>(I) : W;  // workers with items; their starts are distinct
@@ -407,7 +407,7 @@ decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tab
     }
     return;
   }
-  for (int c = tid; c < W; c += kPlanThreads) ws.warp_flag[c * kFlagStride] = 0;
+  for (int c = tid; c < flags; c += kPlanThreads) ws.warp_flag[c * kFlagStride] = 0;
   for (int w = Wp + tid; w <= W; w += kPlanThreads) ws.warp_rec[3 * w] = make_int4(U, 0, 0, 0);  // empty ranges
   for (int w = Wm + tid; w < W; w += kPlanThreads) ws.merge_rec[w] = make_int4(S, 0, 0, 0);      // no merge items
 
@@ -501,7 +501,7 @@ decode_plan_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tab
 constexpr int kListThreads = 64;
 __global__ void __launch_bounds__(kListThreads)
 plan_lists_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tables, int B, int Hkv, int G, int table_stride,
-                  int W, int unit_cost, WsPtrs ws, const PlanScan* scan) {
+                  int W, int flags, int unit_cost, WsPtrs ws, const PlanScan* scan) {
   pdl_wait_primary();
   const int tid = threadIdx.x;
   const long long I = scan->items, MI = scan->merge_items;
@@ -511,9 +511,9 @@ plan_lists_kernel(const int* __restrict__ seq_lens, const int* __restrict__ tabl
   const int Wp = I < W ? static_cast<int>(I) : W;
   const int Wm = MI < W ? static_cast<int>(MI) : W;
   const int cap = table_stride * kBlockTokens, P = B * Hkv;
-  for (int w = blockIdx.x * kListThreads + tid; w <= W; w += gridDim.x * kListThreads) {
-    if (w < W) ws.warp_flag[w * kFlagStride] = 0;
-    if (w >= Wp) ws.warp_rec[3 * w] = make_int4(U, 0, 0, 0);
+  for (int w = blockIdx.x * kListThreads + tid; w <= max(W, flags); w += gridDim.x * kListThreads) {
+    if (w < flags) ws.warp_flag[w * kFlagStride] = 0;
+    if (w >= Wp && w <= W) ws.warp_rec[3 * w] = make_int4(U, 0, 0, 0);
     if (w >= Wm && w < W) ws.merge_rec[w] = make_int4(S, 0, 0, 0);
   }
   const EqualCuts wk(I, Wp), mk(MI, Wm);
@@ -1615,7 +1615,7 @@ int check_attn_int4(int max_warps) {
     }
     ctas[dev] = n;
   }
-  if (num_sms() * SL::kWarps > max_warps)
+  if (num_sms() * (SL::kWarps + 1) > max_warps)
     return set_error(AEG_ERR_UNSUPPORTED, "decode_int4: %d worker warps exceed the workspace's %d", num_sms() * SL::kWarps,
                      max_warps);
   return AEG_OK;
@@ -1917,16 +1917,19 @@ int decode_int4(void* out, int64_t out_stride, const void* q, int64_t q_stride, 
 // Plans on `stream`: scans in one CTA, then the lists over the GPU where the pairs' records fit the
 // partial-result area; else (far more pairs than workers) all of it in one CTA.
 int launch_plan(const char* what, const int32_t* seq_lens, const int32_t* block_tables, int B, int Hkv, int G,
-                int table_stride, int W, int unit_cost, void* workspace, const WsLayout& L, cudaStream_t stream) {
+                int table_stride, int W, int flags, int unit_cost, void* workspace, const WsLayout& L,
+                cudaStream_t stream) {
   const WsPtrs ws = ws_ptrs(workspace, L);
   PlanScan* scan = reinterpret_cast<PlanScan*>(ws.part_ml);
   const int64_t P = int64_t(B) * Hkv;
   if (P == 0 || sizeof(PlanScan) + sizeof(PlanPair) * P > L.total - L.part_ml) {
-    decode_plan_kernel<false><<<1, kPlanThreads, 0, stream>>>(seq_lens, block_tables, B, Hkv, G, table_stride, W, unit_cost, ws, scan);
+    decode_plan_kernel<false><<<1, kPlanThreads, 0, stream>>>(seq_lens, block_tables, B, Hkv, G, table_stride, W, flags,
+                                                                  unit_cost, ws, scan);
     AEG_CHECK_LAUNCH(what);
     return AEG_OK;
   }
-  decode_plan_kernel<true><<<1, kPlanThreads, 0, stream>>>(seq_lens, block_tables, B, Hkv, G, table_stride, W, unit_cost, ws, scan);
+  decode_plan_kernel<true><<<1, kPlanThreads, 0, stream>>>(seq_lens, block_tables, B, Hkv, G, table_stride, W, flags,
+                                                                  unit_cost, ws, scan);
   AEG_CHECK_LAUNCH(what);
   cudaLaunchAttribute attr[1] = {pdl_attr()};
   cudaLaunchConfig_t cfg{};
@@ -1936,8 +1939,8 @@ int launch_plan(const char* what, const int32_t* seq_lens, const int32_t* block_
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   AEG_CHECK_CUDA(cudaLaunchKernelEx(&cfg, plan_lists_kernel, static_cast<const int*>(seq_lens),
-                                    static_cast<const int*>(block_tables), B, Hkv, G, table_stride, W, unit_cost,
-                                    ws, static_cast<const PlanScan*>(scan)));
+                                    static_cast<const int*>(block_tables), B, Hkv, G, table_stride, W, flags,
+                                    unit_cost, ws, static_cast<const PlanScan*>(scan)));
   return AEG_OK;
 }
 
@@ -1951,9 +1954,10 @@ int plan_common(const char* what, void* workspace, size_t workspace_bytes, const
   AEG_CHECK_ARG(B == 0 || (seq_lens != nullptr && block_tables != nullptr), "%s: seq_lens/block_tables is NULL", what);
   AEG_CHECK_ARG(aligned(seq_lens, 4) && aligned(block_tables, 4), "%s: int32 arrays must be aligned", what);
   const int W = int4 ? worker_warps_int4(Hq / Hkv) : worker_warps(Hq / Hkv);
-  if (W > L.max_warps)
+  const int flags = int4 ? W + num_sms() : W;  // a flag per worker; over a 4-bit cache one per CTA too
+  if (flags > L.max_warps)
     return set_error(AEG_ERR_UNSUPPORTED, "%s: %d worker warps exceed the workspace's %d", what, W, L.max_warps);
-  const int launched = launch_plan(what, seq_lens, block_tables, B, Hkv, Hq / Hkv, table_stride, W,
+  const int launched = launch_plan(what, seq_lens, block_tables, B, Hkv, Hq / Hkv, table_stride, W, flags,
                                    int4 ? kUnitCostInt4 : kUnitCost, workspace, L,
                                    static_cast<cudaStream_t>(stream));
   if (launched != AEG_OK) return launched;
@@ -2118,7 +2122,7 @@ int aeg_paged_attn_decode_noalloc(void* out, int64_t out_stride, const void* q, 
   bool waited = false;
   st = order.enter(s, &waited);
   if (st != AEG_OK) return st;
-  st = aeg::launch_plan("decode_plan (noalloc)", seq_lens, block_tables, B, Hkv, Hq / Hkv, table_stride, W, aeg::kUnitCost,
+  st = aeg::launch_plan("decode_plan (noalloc)", seq_lens, block_tables, B, Hkv, Hq / Hkv, table_stride, W, W, aeg::kUnitCost,
                         scratch, L, s);
   if (st != AEG_OK) return st;
   dl.prm.plan_ready = 0;  // the plan kernel directly precedes this launch: read it after the wait

@@ -59,7 +59,8 @@ struct Int4Smem {
   static constexpr int kRecord = (kTokens + 4 * kStages + 15) / 16 * 16;
   static constexpr int kMeta = kRecord + 16;
   static constexpr int kOffMeta = kWarps * kPerWarp;
-  static constexpr size_t kDynamic = size_t(kOffMeta) + kWarps * kMeta + 128;  // + alignment slack
+  static constexpr int kOffDone = kOffMeta + kWarps * kMeta;     // workers that have published
+  static constexpr size_t kDynamic = size_t(kOffDone) + 16 + 128;  // + alignment slack
   static_assert(kPerWarp % 128 == 0 && kDynamic <= 232448, "ring alignment and capacity");
 };
 
@@ -127,6 +128,11 @@ __device__ __forceinline__ void mbar_arrive_after(uint64_t* bar, uint32_t value)
   asm volatile("{\n\t.reg .b32 t;\n\tand.b32 t, %1, 0;\n\tadd.u32 t, t, %0;\n\t"
                "mbarrier.arrive.shared::cta.b64 _, [t];\n\t}" ::"r"(smem_u32(bar)), "r"(value)
                : "memory");
+}
+__device__ __forceinline__ int atom_add_acq_rel_cta(int* p, int v) {
+  int old;
+  asm volatile("atom.acq_rel.cta.shared::cta.add.s32 %0, [%1], %2;" : "=r"(old) : "r"(smem_u32(p)), "r"(v) : "memory");
+  return old;
 }
 __device__ __forceinline__ uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 __device__ __forceinline__ uint2 lds64(const uint8_t* p) { return *reinterpret_cast<const uint2*>(p); }
@@ -356,6 +362,8 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
+  int* const done = reinterpret_cast<int*>(smem + SL::kOffDone);
+  if (threadIdx.x == 0) *done = 0;
   if (warp < kW && lane == 0) {
     const Int4Worker<NT> w(smem, warp);
     for (int s = 0; s < SL::kBars; ++s) mbar_init(&w.full[s], 1);
@@ -773,7 +781,12 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
   const int4 none = make_int4(-1, 0, (1 | (1 << 8)) << 16, 0);
   int4 me = (share_ok && share.z > 0 && entry < n_entries) ? p.ws.split_pairs[entry] : none;
   __syncwarp();
-  if (lane == 0) st_release_gpu(&p.ws.warp_flag[gw * kFlagStride], stamp);
+  if (lane == 0) {
+    st_release_gpu(&p.ws.warp_flag[gw * kFlagStride], stamp);
+    // The CTA's last worker to publish stamps the CTA's flag for all of them.
+    if (atom_add_acq_rel_cta(done, 1) == kW - 1)
+      st_release_gpu(&p.ws.warp_flag[(total_warps + static_cast<int>(blockIdx.x)) * kFlagStride], stamp);
+  }
   int ready_entry = -1;
   if (share_ok) {
     for (int left = share.z; left > 0; --left) {
@@ -788,13 +801,16 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
       }
       if (ready_entry != entry) {
         const int w0 = me.w & 0xffff, nw = me.w >> 16;
-        // 32 flags at a time (asking for all of a long pair's 200 in one round trip, with a fence behind it,
-        // took 4 us longer: the polls of hundreds of warps delay the stamps themselves).
+        // A worker's flag for each of up to 32 pieces; more of them (a pair of 65,536 tokens has 200) wait
+        // for their CTAs' flags, 32 at a time (asking for 200 workers' flags at once delayed the stamps
+        // themselves, 32 at a time cost 7 round trips).
+        const bool by_cta = nw > 32;
+        const int f0 = by_cta ? total_warps + w0 / kW : w0;
+        const int nf = by_cta ? (w0 + nw - 1) / kW - w0 / kW + 1 : nw;
         int ok = 1;
-        for (int i = 0; i < nw && ok; i += 32) {
-          const int ww = w0 + i + lane;
-          ok = __all_sync(0xffffffffu,
-                          i + lane >= nw || ww == gw || flag_wait(&p.ws.warp_flag[ww * kFlagStride], stamp));
+        for (int i = 0; i < nf && ok; i += 32) {
+          const int f = f0 + i + lane;
+          ok = __all_sync(0xffffffffu, i + lane >= nf || f == gw || flag_wait(&p.ws.warp_flag[f * kFlagStride], stamp));
         }
         __syncwarp();
         if (!ok) {
