@@ -8,22 +8,22 @@
 //       q . K = sum over groups of  s (q . c) + m (sum of q)
 //       sum_t p_t V_t = sum_t (p_t s_t) c_t + sum_t p_t m_t
 //     so the codes go to the tensor cores as they are, exactly, and scales and minima meet them
-//     in fp32. A code becomes a 16-bit float with one AND-OR: a nibble under the exponent of a power
-//     of two B reads as B + c, and the constant is taken out with the minima (m - B s in place of
-//     m), in fp32. B is 64 or 128 for the keys, where it is out again after four MMAs, and 16 for
-//     the values (see the fold below).
-//   * S^T = K Q^T as in the 16-bit kernel (16 tokens x 8 heads of the group, m16n8k16), in the
-//     query's own type. A lane's codes of a token are one 16-byte load; which dim sits where in the
-//     contraction is free as long as the query fragments follow.
+//     in fp32. A code becomes an fp16 number with one AND-OR: a nibble under the exponent of 64 reads
+//     as 64 + c, and the constant is taken out with the keys' minima (m - 64 s in place of m) in fp32;
+//     of the values, see the fold below.
+//   * S^T = K Q^T as in the 16-bit kernel (16 tokens x 8 heads of the group, m16n8k16), in fp16 for bf16
+//     queries too, scaled by a power of two. A lane's codes of a token are one 16-byte load; which dim
+//     sits where in the contraction is free as long as the query fragments follow.
 //   * O^T += V^T P^T with codes and P * s as fp16, P * s brought to within 2^15 by a power of two that
 //     follows the largest scale the warp has met: 11 bits for everything down to 2^-23 of the
 //     largest product (bf16 would keep 8 and need a second MMA for the rest). Token pairs share a
 //     32-bit word, so that the transposed fragment comes out of the same AND-OR without a
 //     transposing load. sum p m is 4 FMAs a token and lane.
-//   * The tensor cores cut off what an addition pushes out of the accumulator, always downwards, so
-//     a sum that carries 16 sum(p s) along drifts with its length (at B = 128 the error of 4096
-//     tokens was 2.5 times that of the output's own rounding). Every kFold tiles the constant's
-//     share is therefore taken out of O, which leaves sums of the size of the result.
+//   * The constant multiplies the rounded P * s, so its share is summed from those (one more MMA a
+//     group, with ones) and cancels exactly; what remains is sum (P s)(c - 8) and, in fp32, sum p (m + 8 s).
+//     The tensor cores cut off what an addition pushes out of the accumulator, always downwards, so a sum
+//     that carries the constant along drifts with its length (128 sum(p s) over 4096 tokens: 2.5 times
+//     the error of the output's own rounding). So it is taken out of O every kFold tiles.
 //   * The running maximum moves only when a score exceeds it by kSlack (log2 units): sums are fp32, and
 //     most tiles need one vote instead of a reduction over the tokens and a rescaling of O.
 //   * One warp of the CTA requests the tiles of all others, a lane for each, so that walking the units
@@ -31,9 +31,9 @@
 //
 // What bounds it, per layer inside a graph of layers (and the 16-bit kernel on the same lengths):
 //   4 sequences of 17..300 tokens, 28/4 heads fp16       8.1 us (7.1)   a chain of round trips
-//   64 of lognormal(5.5, 1) tokens, 28/4 heads fp16     10.9 us (13.0)
+//   64 of lognormal(5.5, 1) tokens, 28/4 heads fp16     10.3 us (13.0)
 //   256 of lognormal(6, 1) tokens, 32/4 heads bf16      33.0 us (58.0)  2.5 TB/s of K/V
-//   2 of 40,001..65,535 tokens, 32/4 heads bf16         29.6 us (46.7)
+//   2 of 40,001..65,535 tokens, 32/4 heads bf16         27.4 us (46.7)
 //   16 of 2048..4096 tokens, 40/40 heads fp16           76.9 us (177)   3.8 TB/s
 // Streaming alone (nothing computed) takes 60 us of the last one, computing alone about as long as both
 // together: at 4.5 bits an element the work per byte is 3.6 times that of the 16-bit kernel, ~330
@@ -57,7 +57,7 @@ struct Int4Smem {
   static constexpr int kBars = 2 * kStages + 2;
   static constexpr int kTokens = 8 * kBars;
   static constexpr int kRecord = (kTokens + 4 * kStages + 15) / 16 * 16;
-  static constexpr int kMeta = kRecord + 16;
+  static constexpr int kMeta = kRecord + 32;
   static constexpr int kOffMeta = kWarps * kPerWarp;
   static constexpr int kOffDone = kOffMeta + kWarps * kMeta;     // workers that have published
   static constexpr size_t kDynamic = size_t(kOffDone) + 16 + 128;  // + alignment slack
@@ -96,7 +96,6 @@ template <typename T>
 constexpr float kScaleLeast = std::is_same<T, __half>::value ? 0x1p-14f : 0x1p-100f;  // smaller ones count as this
 template <typename T>
 constexpr uint32_t kScaleMantissa = std::is_same<T, __half>::value ? 0x3ffu : 0x7fu;
-constexpr float kValueMiddle = 8.f;
 
 // Products, transpositions and shared loads that the compiler may move among one another (those of
 // aeg_common.cuh are volatile and keep their order): a tile's chains overlap only if it does. The
@@ -122,12 +121,6 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
   return done != 0;
-}
-// Arrives on `bar` once `value` is known.
-__device__ __forceinline__ void mbar_arrive_after(uint64_t* bar, uint32_t value) {
-  asm volatile("{\n\t.reg .b32 t;\n\tand.b32 t, %1, 0;\n\tadd.u32 t, t, %0;\n\t"
-               "mbarrier.arrive.shared::cta.b64 _, [t];\n\t}" ::"r"(smem_u32(bar)), "r"(value)
-               : "memory");
 }
 __device__ __forceinline__ int atom_add_acq_rel_cta(int* p, int v) {
   int old;
@@ -157,6 +150,7 @@ struct Int4Worker {
   uint64_t* qempty;
   int* tokens;      // valid tokens of the stage's tile
   int4* record;     // {tiles (-1: no more units), partial slot or -1, sequence, KV head}
+  volatile uint32_t* seen;
   __device__ Int4Worker(uint8_t* smem, int w) {
     ring = smem + w * SL::kPerWarp;
     q = ring + SL::kRing;
@@ -167,6 +161,7 @@ struct Int4Worker {
     qempty = qfull + 1;
     tokens = reinterpret_cast<int*>(meta + SL::kTokens);
     record = reinterpret_cast<int4*>(meta + SL::kRecord);
+    seen = reinterpret_cast<uint32_t*>(meta + SL::kRecord + 16);
   }
 };
 
@@ -398,11 +393,11 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
   else if (lane == 2) mr.x = ld_hint(&p.ws.header[kHdrSplitPairs], keep);
   else if (lane == 3) mr.x = ld_relaxed_gpu(&p.ws.warp_flag[gw * kFlagStride]);
 
-  bool lost = false;  // a wait ran out: this warp's results are not complete
+  bool lost = false;  // a wait ran out (the lanes agree on it): this warp's results are not complete
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return;
-    if (lost || !mbar_wait_bounded(bar, parity, kWaitLimitNs)) {
-      if (!lost && lane == 0) atomicOr(&g_deverr_attn, AEG_DEVERR_WAIT_TIMEOUT);
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return;
+    if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, kWaitLimitNs))) {
+      if (lane == 0) atomicOr(&g_deverr_attn, AEG_DEVERR_WAIT_TIMEOUT);
       lost = true;
     }
   };
@@ -510,7 +505,8 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
       sc[nt][0] = __shfl_sync(0xffffffffu, back, 8 * quad);
       sc[nt][1] = __shfl_sync(0xffffffffu, back, 8 * quad + 4);
     }
-    // The slot is free once every lane's values have arrived: a vote on them needs them all.
+    // The slot is free once every lane's values have arrived: the vote stored before the arrival needs
+    // them all.
     if (!first) {
       uint32_t dep = 0;
 #pragma unroll
@@ -518,7 +514,10 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) dep |= qf[nt][ks][0] | qf[nt][ks][1];
       const uint32_t any = __ballot_sync(0xffffffffu, dep != 0);
-      if (lane == 0) mbar_arrive_after(wk.qempty, any);
+      if (lane == 0) {
+        *wk.seen = any;
+        mbar_arrive(wk.qempty);
+      }
     }
     first = false;
 

@@ -192,7 +192,7 @@ extern "C" int aeg_rotary_multi_axis(void* q_out, int64_t q_out_stride, void* k_
   AEG_CHECK_ARG(q_stride >= int64_t(Hq) * D && q_out_stride >= int64_t(Hq) * D && k_stride >= int64_t(Hkv) * D &&
                     k_out_stride >= int64_t(Hkv) * D,
                 "rotary_multi_axis: token stride smaller than heads*D");
-  AEG_CHECK_ARG(axes == 1 || axis_stride >= T, "rotary_multi_axis: axis stride smaller than the token count");
+  AEG_CHECK_ARG(axis_stride >= 0, "rotary_multi_axis: negative axis stride");
   AEG_CHECK_ARG(aeg::aligned(q, 2) && aeg::aligned(k, 2) && aeg::aligned(q_out, 2) && aeg::aligned(k_out, 2) &&
                     aeg::aligned(positions, 8) && aeg::aligned(inv_freq, 4),
                 "rotary_multi_axis: misaligned pointer");

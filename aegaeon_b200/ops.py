@@ -678,7 +678,8 @@ def rotary_multi_axis(query: torch.Tensor, key: torch.Tensor, positions: torch.T
     """Rotates ``query`` ``[T, Hq, D]`` and ``key`` ``[T, Hkv, D]`` (fp16 or bf16, any token stride) by
     positions with up to four axes (time, height, width of image and video tokens).
 
-    ``positions`` int64 ``[axes, T]`` (``[T]`` for one axis, as ``prepare_step_inputs`` gives them),
+    ``positions`` int64 ``[axes, T]`` (``[T]`` for one axis, as ``prepare_step_inputs`` gives them; text
+    tokens on several axes may be ``positions.expand(axes, -1)``),
     ``inv_freq`` float32 ``[half]``; ``sections[a]`` frequencies belong to axis a: one section after
     another, or with ``interleaved=True`` dealt to the axes in turn until an axis has its number. Pairs
     are dims (i, i + half); dims from ``2 * half`` on are copied. ``scaling`` multiplies the rotated
@@ -701,7 +702,7 @@ def rotary_multi_axis(query: torch.Tensor, key: torch.Tensor, positions: torch.T
     if positions.dtype != torch.int64 or positions.shape != (axes, T):
         raise ValueError(f"positions must be int64 [{axes}, {T}]")
     axis_stride, step = positions.stride()
-    if (step != 1 and T > 1) or axis_stride < T:
+    if step != 1 and T > 1:
         positions = positions.contiguous()
         axis_stride = T
     if inv_freq.dtype != torch.float32 or inv_freq.shape != (half,):

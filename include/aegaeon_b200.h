@@ -415,7 +415,7 @@ AEG_API int aeg_paged_attn_decode_int4(void* out, int64_t out_stride, const void
  * model's rotary embedding through vLLM (aegaeon/aegaeon/worker.py:517-523).
  *
  * For i < half with a = axis_of[i] (HOST bytes, a < axes <= 4) and theta = positions[a][t] *
- * inv_freq[i] (positions: DEVICE int64 [axes] rows `axis_stride` apart; inv_freq: DEVICE float):
+ * inv_freq[i] (positions: DEVICE int64 [axes] rows `axis_stride` >= 0 apart; inv_freq: DEVICE float):
  *   out[t][h][i]        = scaling * (x[t][h][i] cos(theta) - x[t][h][i + half] sin(theta))
  *   out[t][h][i + half] = scaling * (x[t][h][i + half] cos(theta) + x[t][h][i] sin(theta))
  * for every head h of q [T, Hq, D] and k [T, Hkv, D] (token strides in elements, Hkv may be 0); dims

@@ -79,6 +79,9 @@ def test_sliced_positions_empty_call_and_refusals(cuda_device):
     assert torch.equal(got, ops.rotary_multi_axis(x, x, wide[:, 2:5].contiguous(), inv, (16, 24, 24))[0])
     got = ops.rotary_multi_axis(x, x, wide.T[2:5].T, inv, (16, 24, 24))[0]
     assert torch.equal(got, ops.rotary_multi_axis(x, x, wide[:, 2:5], inv, (16, 24, 24))[0])
+    one = wide[0, 2:5]
+    got = ops.rotary_multi_axis(x, x, one.expand(3, -1), inv, (16, 24, 24))[0]
+    assert torch.equal(got, ops.rotary_multi_axis(x, x, one, inv, (64,))[0])
     got = ops.rotary_multi_axis(x[:0], x[:0], wide[:, :0], inv, (16, 24, 24))
     assert got[0].shape == (0, 2, 128)
     pos = wide[:, :3]

@@ -161,7 +161,7 @@ def test_rotary_refuses_on_the_host():
     assert call(q=None) == INVAL and call(k=None) == INVAL and call(pos=None) == INVAL and call(inv=None) == INVAL
     assert call(ax=None) == INVAL
     assert call(qs=1000) == INVAL and call(qos=1000) == INVAL and call(ks=255) == INVAL and call(kos=255) == INVAL
-    assert call(ps=3) == INVAL and call(q=p + 1) == INVAL and call(pos=p + 4) == INVAL
+    assert call(ps=-1) == INVAL and call(q=p + 1) == INVAL and call(pos=p + 4) == INVAL
 
 
 def test_shared_block_calls_refuse_on_the_host():
