@@ -919,9 +919,11 @@ class DecodePlan:
 
     def matches(self, B: int, Hq: int, Hkv: int, D: int, block_table: torch.Tensor, seq_lens: torch.Tensor,
                 cache: str = "auto") -> bool:
+        tables, lens = self.block_tables, self.seq_lens
         return ((self.batch, self.num_q_heads, self.num_kv_heads, self.head_dim, self.cache) == (B, Hq, Hkv, D, cache)
-                and self.block_tables is not None and self.block_tables.data_ptr() == block_table.data_ptr()
-                and self.seq_lens.data_ptr() == seq_lens.data_ptr() and self.table_width == block_table.size(1))
+                and tables is not None and (tables is block_table or tables.data_ptr() == block_table.data_ptr())
+                and (lens is seq_lens or lens.data_ptr() == seq_lens.data_ptr())
+                and self.table_width == block_table.size(1))
 
 
 def flash_attn_decode(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -1085,8 +1087,43 @@ def paged_attention_decode_int4(out: torch.Tensor, query: torch.Tensor, kv_cache
     this stream writes neither this layer's blocks nor the block tables (so not right after the
     layer's ``reshape_and_cache_int4``).
     """
+    # A decode loop makes this call for every layer of every step, so its usual form is recognised in one
+    # expression; anything else is checked piece by piece (and refused, or brought into that form).
+    try:
+        B, Hq, D = shape = query.shape
+        N, L, Hkv, tile = kv_cache.shape
+        q_stride, q1, q2 = query.stride()
+        out_stride, o1, o2 = out.stride()
+        t_stride, t1 = block_tables.stride()
+        dtype, index, i32 = query.dtype, query.get_device(), torch.int32
+        usual = (plan is not None and q1 == D == o1 and q2 == 1 == o2 == t1 and tile == INT4_TILE and 0 <= layer < L
+                 and kv_cache.dtype is dtype and out.dtype is dtype and block_tables.dtype is i32 and seq_lens.dtype is i32
+                 and 0 <= index == kv_cache.get_device() == block_tables.get_device() == seq_lens.get_device()
+                 == out.get_device() == plan.workspace.get_device()
+                 and out.shape == shape and seq_lens.shape == (B,) and dtype in _DTYPES and kv_cache.is_contiguous()
+                 and seq_lens.is_contiguous() and plan.matches(B, Hq, Hkv, D, block_tables, seq_lens, "int4"))
+    except (AttributeError, TypeError, ValueError, IndexError):
+        usual = False
+    if not usual:
+        block_tables, seq_lens, plan = _check_attention_int4(out, query, kv_cache, layer, block_tables, seq_lens, plan)
+        if plan is None:  # an empty batch
+            return
+        (B, Hq, D), (N, L, Hkv, tile) = query.shape, kv_cache.shape
+        q_stride, out_stride, t_stride = query.stride(0), out.stride(0), block_tables.stride(0)
+        dtype, index = query.dtype, query.get_device()
+    ws = plan.workspace
+    head = Hkv * INT4_TILE
+    _launch(index, "paged_attention_decode_int4", lib.aeg_paged_attn_decode_int4, out.data_ptr(), out_stride,
+            query.data_ptr(), q_stride, kv_cache.data_ptr() + 2 * layer * head, L * head, N, block_tables.data_ptr(), t_stride,
+            seq_lens.data_ptr(), B, Hq, Hkv, D, float(scale), _DTYPES[dtype], ws.data_ptr(), ws.numel(),
+            AEG_DECODE_PREFETCH if prefetch else 0)
+
+
+def _check_attention_int4(out, query, kv_cache, layer, block_tables, seq_lens, plan):
+    """Checks every argument of ``paged_attention_decode_int4``; returns contiguous tables and lengths and
+    a plan for them (None for an empty batch)."""
     B, Hq, D = shape = _token_rows(query, "query", "[B, Hq, D]")
-    base, block_stride, N, Hkv = _int4_layer(kv_cache, layer)
+    Hkv = _int4_layer(kv_cache, layer)[3]
     dtype = query.dtype
     if dtype != kv_cache.dtype:
         raise ValueError(f"query dtype {dtype} differs from cache dtype {kv_cache.dtype}")
@@ -1102,20 +1139,15 @@ def paged_attention_decode_int4(out: torch.Tensor, query: torch.Tensor, kv_cache
     if _token_rows(out, "out", "query's shape") != shape or out.dtype != dtype:
         raise ValueError("out must match query's shape and dtype")
     index = query.get_device()
-    if not (index == kv_cache.get_device() == block_tables.get_device() == seq_lens.get_device() == out.get_device()):
-        _on_devices(index, dict(kv_cache=kv_cache, block_tables=block_tables, seq_lens=seq_lens, out=out))
+    for name, t in (("kv_cache", kv_cache), ("block_tables", block_tables), ("seq_lens", seq_lens), ("out", out)):
+        _on_device(index, t, name)
     if B == 0:
-        return
+        return block_tables, seq_lens, None
     if block_tables.size(1) == 0:
         raise ValueError("block_tables has no columns")
     if plan is None:
         plan = DecodePlan(B, Hq, Hkv, D, query.device, cache="int4").plan(seq_lens, block_tables)
     elif not plan.matches(B, Hq, Hkv, D, block_tables, seq_lens, "int4"):
         raise ValueError("plan was built for a different batch / head layout / block tables / sequence lengths / cache")
-    ws = plan.workspace
-    if ws.get_device() != index:
-        _on_device(index, ws, "plan workspace")
-    _launch(index, "paged_attention_decode_int4", lib.aeg_paged_attn_decode_int4, out.data_ptr(), out.stride(0),
-            query.data_ptr(), query.stride(0), base, block_stride, N, block_tables.data_ptr(), block_tables.stride(0),
-            seq_lens.data_ptr(), B, Hq, Hkv, D, float(scale), _DTYPES[dtype], ws.data_ptr(), ws.numel(),
-            AEG_DECODE_PREFETCH if prefetch else 0)
+    _on_device(index, plan.workspace, "plan workspace")
+    return block_tables, seq_lens, plan
