@@ -55,9 +55,9 @@ class DecodeStep:
 
     @property
     def launches_per_step(self) -> int:
-        """Kernels one step launches: the plan, then per layer the fused cache-write/attention
-        launch (fused) or the cache write and the attention (unfused)."""
-        return 1 + (1 if self.fused else 2) * self.shape.num_layers
+        """Kernels one step launches: the plan's two (scans, then lists), then per layer the fused
+        cache-write/attention launch (fused) or the cache write and the attention (unfused)."""
+        return 2 + (1 if self.fused else 2) * self.shape.num_layers
 
     def run_eager(self) -> None:
         """One step on the current stream, op by op."""
