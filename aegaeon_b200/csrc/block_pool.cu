@@ -109,6 +109,9 @@ struct PoolParams {
   int* seq_lens;
 };
 
+// Pointers are not __restrict__: a load promised to be invariant may be moved ahead of the grid-dependency
+// wait, and the kernel before this one may itself have started early.
+
 // ---- fork --------------------------------------------------------------------------------------
 
 // What fork_plan_kernel leaves for fork_apply_kernel, one per entry: {source row, target row, length
@@ -120,8 +123,8 @@ struct ForkScratch {
 };
 
 __global__ void __launch_bounds__(kPlanThreads, 1)
-fork_plan_kernel(const PoolParams p, const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n, ForkScratch ws,
-                 int* __restrict__ new_blocks) {
+fork_plan_kernel(const PoolParams p, const int64_t* src, const int64_t* dst, int n, ForkScratch ws,
+                 int* new_blocks) {
   __shared__ int s_warp[32];
   pdl_launch_dependents();
   pdl_wait_primary();
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(kCopyThreads) fork_apply_kernel(const PoolPara
 
 // One CTA a row. The row's length is taken with an exchange, so a row named twice is freed once.
 __global__ void __launch_bounds__(kCopyThreads)
-free_kernel(const PoolParams p, const int64_t* __restrict__ row_ids) {
+free_kernel(const PoolParams p, const int64_t* row_ids) {
   __shared__ int s_len;
   pdl_launch_dependents();
   pdl_wait_primary();

@@ -598,27 +598,34 @@ def _int4_layer(kv_cache: torch.Tensor, layer: int) -> tuple[int, int, int, int]
     return kv_cache.data_ptr() + layer * Hkv * INT4_TILE * 2, L * Hkv * INT4_TILE, N, Hkv
 
 
-def _int4_move(fn, what: str, key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, layer: int,
-               slot_mapping: torch.Tensor) -> None:
+def _int4_move(fn, what: str, key: torch.Tensor | None, value: torch.Tensor | None, kv_cache: torch.Tensor, layer: int,
+               slot_mapping: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Moves rows between ``key``/``value`` (new ones when None) and ``slot_mapping``'s slots of ``layer``."""
     base, block_stride, N, Hkv = _int4_layer(kv_cache, layer)
-    shape = _token_rows(key, "key", "[T, Hkv, D]")
-    if _token_rows(value, "value", "[T, Hkv, D]") != shape:
-        raise ValueError("key and value must have the same shape")
-    T, heads, D = shape
-    dtype = kv_cache.dtype
-    if key.dtype != dtype or value.dtype != dtype:
-        raise ValueError(f"key dtype {key.dtype} or value dtype {value.dtype} differs from cache dtype {dtype}")
-    if heads != Hkv:
-        raise ValueError(f"kv_cache holds {Hkv} KV heads, not {heads}")
-    _require_cuda(slot_mapping, "slot_mapping")
+    dtype, index = kv_cache.dtype, kv_cache.get_device()
+    _on_device(index, slot_mapping, "slot_mapping")
+    if key is None:
+        T, D = slot_mapping.numel(), 128
+        key = kv_cache.new_empty((T, Hkv, D))
+        value = torch.empty_like(key)
+        k_stride = v_stride = Hkv * D
+    else:
+        T, heads, D = shape = _token_rows(key, "key", "[T, Hkv, D]")
+        if _token_rows(value, "value", "[T, Hkv, D]") != shape:
+            raise ValueError("key and value must have the same shape")
+        if key.dtype != dtype or value.dtype != dtype:
+            raise ValueError(f"key dtype {key.dtype} or value dtype {value.dtype} differs from cache dtype {dtype}")
+        if heads != Hkv:
+            raise ValueError(f"kv_cache holds {Hkv} KV heads, not {heads}")
+        if not (index == key.get_device() == value.get_device()):
+            _on_devices(index, dict(key=key, value=value))
+        k_stride, v_stride = key.stride(0), value.stride(0)
     if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (T,):
         raise ValueError("slot_mapping must be int64 [T]")
     slot_mapping = slot_mapping.contiguous()
-    index = kv_cache.get_device()
-    if not (index == key.get_device() == value.get_device() == slot_mapping.get_device()):
-        _on_devices(index, dict(key=key, value=value, slot_mapping=slot_mapping))
-    _launch(index, what, fn, key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0), base, block_stride, N,
+    _launch(index, what, fn, key.data_ptr(), value.data_ptr(), k_stride, v_stride, base, block_stride, N,
             slot_mapping.data_ptr(), T, Hkv, D, _DTYPES[dtype])
+    return key, value
 
 
 def reshape_and_cache_int4(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, layer: int,
@@ -631,6 +638,7 @@ def reshape_and_cache_int4(key: torch.Tensor, value: torch.Tensor, kv_cache: tor
     minimum`` with a 4-bit code; a group with a NaN or an infinity reads back as NaN. The slots of one
     call must be distinct.
     """
+    _require_cuda(key, "key")
     _int4_move(lib.aeg_reshape_and_cache_int4, "reshape_and_cache_int4", key, value, kv_cache, layer, slot_mapping)
 
 
@@ -641,14 +649,7 @@ def gather_cache_int4(kv_cache: torch.Tensor, layer: int, slot_mapping: torch.Te
     takes over. Slots < 0 give zero rows. ``key``/``value`` receive the result when given."""
     if (key is None) != (value is None):
         raise ValueError("key and value are given together")
-    if key is None:
-        _require_cuda(kv_cache, "kv_cache")
-        _require_cuda(slot_mapping, "slot_mapping")
-        if kv_cache.dim() != 4:
-            raise ValueError(f"kv_cache must be a 4-bit cache (N, L, Hkv, {INT4_TILE})")
-        key, value = kv_cache.new_empty((2, slot_mapping.numel(), kv_cache.size(2), 128)).unbind()
-    _int4_move(lib.aeg_gather_cache_int4, "gather_cache_int4", key, value, kv_cache, layer, slot_mapping)
-    return key, value
+    return _int4_move(lib.aeg_gather_cache_int4, "gather_cache_int4", key, value, kv_cache, layer, slot_mapping)
 
 
 # --------------------------------------------------------------------------------------------
@@ -685,45 +686,66 @@ def rotary_multi_axis(query: torch.Tensor, key: torch.Tensor, positions: torch.T
     are dims (i, i + half); dims from ``2 * half`` on are copied. ``scaling`` multiplies the rotated
     dims. Returns new tensors unless ``query_out``/``key_out`` are given; those may be the inputs.
     """
-    T, Hq, D = _token_rows(query, "query", "[T, Hq, D]")
+    sections = tuple(sections)
+    axis_of = _axis_of(sections, bool(interleaved))
+    axes, half = len(sections), len(axis_of)
+    # The usual form is recognised in one expression; anything else is checked piece by piece.
+    try:
+        T, Hq, D = query.shape
+        kT, Hkv, kD = key.shape
+        q_stride, q1, q2 = query.stride()
+        k_stride, k1, k2 = key.stride()
+        axis_stride, step = positions.stride()
+        dtype, index = query.dtype, query.get_device()
+        usual = (q1 == D == k1 == kD and q2 == 1 == k2 == step and kT == T and dtype in _DTYPES and key.dtype is dtype
+                 and 0 <= index == key.get_device() == positions.get_device() == inv_freq.get_device()
+                 and positions.dtype is torch.int64 and positions.shape == (axes, T)
+                 and inv_freq.dtype is torch.float32 and inv_freq.shape == (half,) and inv_freq.is_contiguous())
+    except (AttributeError, TypeError, ValueError, IndexError):
+        usual = False
+    if not usual:
+        positions, inv_freq = _check_rotary(query, key, positions, inv_freq, axes, half)
+        (T, Hq, D), Hkv = query.shape, key.size(1)
+        q_stride, k_stride, axis_stride = query.stride(0), key.stride(0), positions.stride(0)
+        dtype, index = query.dtype, query.get_device()
+    if query_out is None:
+        query_out = torch.empty_like(query) if query.is_contiguous() else query.new_empty(query.shape)
+    else:
+        _check_rotary_out(index, query_out, query, "query_out")
+    if key_out is None:
+        key_out = torch.empty_like(key) if key.is_contiguous() else key.new_empty(key.shape)
+    else:
+        _check_rotary_out(index, key_out, key, "key_out")
+    _launch(index, "rotary_multi_axis", lib.aeg_rotary_multi_axis, query_out.data_ptr(), query_out.stride(0),
+            key_out.data_ptr(), key_out.stride(0), query.data_ptr(), q_stride, key.data_ptr(), k_stride,
+            positions.data_ptr(), axis_stride, axes, inv_freq.data_ptr(), axis_of, half, float(scaling), T, Hq, Hkv, D,
+            _DTYPES[dtype])
+    return query_out, key_out
+
+
+def _check_rotary(query, key, positions, inv_freq, axes: int, half: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Checks the inputs of ``rotary_multi_axis``; returns positions ``[axes, T]`` with contiguous rows and
+    contiguous frequencies."""
+    T, _, D = _token_rows(query, "query", "[T, Hq, D]")
     k_shape = _token_rows(key, "key", "[T, Hkv, D]")
-    dtype = query.dtype
-    if dtype not in _DTYPES or key.dtype != dtype:
+    if query.dtype not in _DTYPES or key.dtype != query.dtype:
         raise ValueError("query and key must share an fp16 or bf16 dtype")
     if k_shape[0] != T or k_shape[2] != D:
         raise ValueError("query and key must have the same tokens and head_dim")
-    sections = tuple(sections)
-    axis_of = _axis_of(sections, bool(interleaved))
-    half, axes = len(axis_of), len(sections)
     _require_cuda(positions, "positions")
     _require_cuda(inv_freq, "inv_freq")
     if positions.dim() == 1:
         positions = positions.unsqueeze(0)
     if positions.dtype != torch.int64 or positions.shape != (axes, T):
         raise ValueError(f"positions must be int64 [{axes}, {T}]")
-    axis_stride, step = positions.stride()
-    if step != 1 and T > 1:
-        positions = positions.contiguous()
-        axis_stride = T
     if inv_freq.dtype != torch.float32 or inv_freq.shape != (half,):
         raise ValueError(f"inv_freq must be float32 [{half}], one per frequency of the sections")
-    inv_freq = inv_freq.contiguous()
     index = query.get_device()
-    if not (index == key.get_device() == positions.get_device() == inv_freq.get_device()):
-        _on_devices(index, dict(key=key, positions=positions, inv_freq=inv_freq))
-    if query_out is None:
-        query_out = torch.empty_like(query) if query.is_contiguous() else query.new_empty(query.shape)
-    else:
-        _check_rotary_out(index, query_out, query, "query_out")
-    if key_out is None:
-        key_out = torch.empty_like(key) if key.is_contiguous() else key.new_empty(k_shape)
-    else:
-        _check_rotary_out(index, key_out, key, "key_out")
-    _launch(index, "rotary_multi_axis", lib.aeg_rotary_multi_axis, query_out.data_ptr(), query_out.stride(0),
-            key_out.data_ptr(), key_out.stride(0), query.data_ptr(), query.stride(0), key.data_ptr(), key.stride(0),
-            positions.data_ptr(), axis_stride, axes, inv_freq.data_ptr(), axis_of, half, float(scaling), T, Hq, k_shape[1], D,
-            _DTYPES[dtype])
-    return query_out, key_out
+    for name, t in (("key", key), ("positions", positions), ("inv_freq", inv_freq)):
+        _on_device(index, t, name)
+    if positions.stride(1) != 1 and T > 1:
+        positions = positions.contiguous()
+    return positions, inv_freq.contiguous()
 
 
 def _check_rotary_out(index: int, out: torch.Tensor, src: torch.Tensor, name: str) -> None:

@@ -435,7 +435,8 @@ AEG_API int aeg_rotary_multi_axis(void* q_out, int64_t q_out_stride, void* k_out
  *   ref_counts    int32 [num_blocks]      table rows that hold the block; 0 = free
  *   block_tables  int32 [rows, table_stride], seq_lens int32 [rows]: row r holds the first
  *                 ceil(seq_lens[r] / 16) entries of its table row; length 0 = an empty row
- * Free blocks are taken lowest id first, in the order of the call's entries.
+ * Free blocks are taken lowest id first, in the order of the call's entries. Calls on one state are
+ * ordered by the caller (one stream, or streams that wait for one another).
  *
  * aeg_fork_blocks: for i < n, the empty row d_dst_rows[i] becomes a copy of row d_src_rows[i] (its
  * length, its blocks), sharing every full block; a partly filled last block, which both rows go on

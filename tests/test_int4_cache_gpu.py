@@ -142,7 +142,7 @@ def test_empty_calls_and_refusals(cuda_device):
     assert ops.gather_cache_int4(cache, 0, no_slots)[0].shape == (0, 4, 128)
     row = torch.zeros(1, 4, 128, dtype=torch.float16, device=cuda_device)
     slot = torch.zeros(1, dtype=torch.int64, device=cuda_device)
-    for bad in (dict(key=row.bfloat16()), dict(key=row[:, :2]), dict(slots=slot.int()), dict(slots=slot.cpu()), dict(layer=1),
+    for bad in (dict(key=None), dict(key=row.bfloat16()), dict(key=row[:, :2]), dict(slots=slot.int()), dict(slots=slot.cpu()), dict(layer=1),
                 dict(cache=cache[..., :1024]), dict(cache=cache.float()), dict(key=row.double()), dict(slots=slot.repeat(2))):
         a = dict(dict(key=row, cache=cache, layer=0, slots=slot), **bad)
         with pytest.raises(ValueError):

@@ -208,6 +208,8 @@ def test_wrappers_refuse_host_tensors():
     with pytest.raises(ValueError, match="CUDA"):
         ops.reshape_and_cache_int4(row, row, kv, 0, torch.zeros(2, dtype=torch.int64))
     with pytest.raises(ValueError, match="CUDA"):
+        ops.reshape_and_cache_int4(None, None, kv, 0, torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(ValueError, match="CUDA"):
         ops.gather_cache_int4(kv, 0, torch.zeros(2, dtype=torch.int64))
     with pytest.raises(ValueError, match="CUDA"):
         ops.rotary_multi_axis(row, row, torch.zeros(3, 2, dtype=torch.int64), torch.zeros(64), [64, 0, 0])
