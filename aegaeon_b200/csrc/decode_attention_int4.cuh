@@ -30,17 +30,19 @@
 //     and the block table costs the computing warps neither instructions nor registers.
 //
 // What bounds it, per layer inside a graph of layers (and the 16-bit kernel on the same lengths):
-//   4 sequences of 17..300 tokens, 28/4 heads fp16       8.1 us (7.1)   a chain of round trips
+//   4 sequences of 17..300 tokens, 28/4 heads fp16       8.3 us (7.1)   a chain of round trips
 //   64 of lognormal(5.5, 1) tokens, 28/4 heads fp16     10.3 us (13.0)
-//   256 of lognormal(6, 1) tokens, 32/4 heads bf16      33.0 us (58.0)  2.5 TB/s of K/V
-//   2 of 40,001..65,535 tokens, 32/4 heads bf16         27.4 us (46.7)
+//   256 of lognormal(6, 1) tokens, 32/4 heads bf16      33.1 us (58.0)  2.5 TB/s of K/V
+//   2 of 40,001..65,535 tokens, 32/4 heads bf16         27.6 us (46.7)
 //   16 of 2048..4096 tokens, 40/40 heads fp16           76.9 us (177)   3.8 TB/s
 // Streaming alone (nothing computed) takes 60 us of the last one, computing alone about as long as both
 // together: at 4.5 bits an element the work per byte is 3.6 times that of the 16-bit kernel, ~330
 // instructions a tile at half the issue rate (three warps a scheduler, 168 registers each). 15 workers of
 // 128 registers, 7 of 255, two tiles at a time in a worker, the next tile's scores ahead of this one's
-// products, 16 % fewer integer instructions: each within 5 % or slower. Start, split merge and the
-// slowest SM take 8 to 14 us of a launch; the next layer's start overlaps most of the first.
+// products, 16 % fewer integer instructions: each within 5 % or slower. Workers that issue their own
+// copies, from a queue of addresses that the spare warp fills: 94 us for the last case, 38 for the third.
+// Start, split merge and the slowest SM take 8 to 14 us of a launch; the next layer's start overlaps most
+// of the first.
 
 template <int NT>
 struct Int4Smem {
