@@ -593,20 +593,25 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
       }
     };
 
-    // Makes room for the scores x and the scales under vtop: the maxima move to the tile's, and what
-    // was summed so far follows.
-    auto make_room = [&](const float (*x)[4], uint32_t vtop) {
-      uint32_t top = vtop;
+    // Makes room for the scores x and the scales of the value pairs vp0, vp1: the maxima move to the tile's,
+    // and what was summed so far follows.
+    auto make_room = [&](const float (*x)[4], const uint2& vp0, const uint2& vp1) {
+      // Of the finite scales alone: NaN needs no room, it makes its own group's result NaN by itself, and the
+      // other group of the head goes on.
+      uint32_t top = 0;
+      for (const uint32_t pair : {vp0.x, vp0.y, vp1.x, vp1.y}) {
+        const uint32_t scale = pair & 0xffffu;
+        if (scale < kScaleInf<T>) top = max(top, scale);
+      }
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
       float grow = 1.f;
-      if (top > vlim && top < kScaleInf<T>) {
-        // The power of two above the scale, kept in range for the tiniest ones. NaN needs no room: it
-        // makes the result NaN by itself.
+      if (top > vlim) {
+        // The power of two above the scale, kept in range for the tiniest ones.
         const float t = fmaxf(unpack2<T>(top).x, kScaleLeast<T>);
         const uint32_t e = __float_as_uint(t) >> 23;  // t in [2^(e - 127), 2^(e - 126))
         const float next = __uint_as_float((253u - e) << 23) * kTop;
-        grow = vlim == 0 ? 1.f : next / vmul;  // nothing but zeros was added before the first scale
+        grow = next / vmul;
         vmul = next;
         vlim = bits16(from_float<T>(t)) | kScaleMantissa<T>;
       }
@@ -660,7 +665,7 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) over = over || fmaxf(x[nt][i], x[nt][i + 2]) > mt_[nt][i];
-      if (__any_sync(0xffffffffu, over)) make_room(x, vtop);
+      if (__any_sync(0xffffffffu, over)) make_room(x, vp0, vp1);
 
       const uint8_t* vcodes = tile + kInt4ValueCodes + quad * 128 + grp * 16;
       const uint4 vc0 = lds128(vcodes), vc1 = lds128(vcodes + 512);
