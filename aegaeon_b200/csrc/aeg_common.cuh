@@ -64,6 +64,13 @@ uint32_t deverr_read_and_clear_prefill(cudaStream_t s, cudaError_t* err);
 uint32_t deverr_read_and_clear_int4(cudaStream_t s, cudaError_t* err);
 uint32_t deverr_read_and_clear_pool(cudaStream_t s, cudaError_t* err);
 
+// Whether an unfused decode attention is the last of this library's launches on `s` that let their successor
+// start early. Such an attention starts only after everything before it, and writes no cache block and no
+// table: a cache write behind it may let the kernel after it start at once, beside both.
+bool follows_attention(cudaStream_t s);
+// Records a launch on `s` that lets its successor start early.
+void note_launch(cudaStream_t s, bool attention);
+
 // ---------------------------------------------------------------------------------------
 // Device helpers.
 
@@ -180,6 +187,20 @@ __device__ __forceinline__ void prefetch_l2(const void* ptr) {
 __device__ __forceinline__ void pdl_wait_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+// Waits for the preceding kernel, then lets the next one launch. In this order whatever starts early runs
+// beside its direct predecessor at most: a decode attention that requests tiles before its own wait relies on
+// what that one kernel writes, and on nothing that ran before it.
+__device__ __forceinline__ void pdl_enter() {
+  pdl_wait_primary();
+  pdl_launch_dependents();
+}
+// The same for a cache write; the next kernel may launch before the wait where the host found that only an
+// attention can still be running then (follows_attention).
+__device__ __forceinline__ void pdl_enter_write(bool early) {
+  if (early) pdl_launch_dependents();
+  pdl_wait_primary();
+  if (!early) pdl_launch_dependents();
 }
 
 // Warp-level tensor-core fragments ------------------------------------------------------

@@ -126,8 +126,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1)
 fork_plan_kernel(const PoolParams p, const int64_t* src, const int64_t* dst, int n, ForkScratch ws,
                  int* new_blocks) {
   __shared__ int s_warp[32];
-  pdl_launch_dependents();
-  pdl_wait_primary();
+  pdl_enter();
   const int tid = threadIdx.x;
   const int cap = p.table_stride * kBlockTokens;
   // Entries in themselves. Lengths are read past the L1 cache: the claims below change them.
@@ -228,8 +227,7 @@ fork_plan_kernel(const PoolParams p, const int64_t* src, const int64_t* dst, int
 
 template <bool kVec>
 __global__ void __launch_bounds__(kCopyThreads) fork_apply_kernel(const PoolParams p, int n, ForkScratch ws) {
-  pdl_launch_dependents();
-  pdl_wait_primary();
+  pdl_enter();
   for (int i = blockIdx.x; i < n; i += gridDim.x) {
     const int4 e = ws.entry[i];
     const int* from = p.tables + static_cast<int64_t>(e.x) * p.table_stride;
@@ -257,8 +255,7 @@ __global__ void __launch_bounds__(kCopyThreads) fork_apply_kernel(const PoolPara
 __global__ void __launch_bounds__(kCopyThreads)
 free_kernel(const PoolParams p, const int64_t* row_ids) {
   __shared__ int s_len;
-  pdl_launch_dependents();
-  pdl_wait_primary();
+  pdl_enter();
   const int64_t row = row_ids[blockIdx.x];
   if (!valid_id(row, p.rows)) {
     if (threadIdx.x == 0) report(AEG_DEVERR_POOL_ENTRY);
@@ -304,8 +301,7 @@ struct CompactOut {
 __global__ void __launch_bounds__(kPlanThreads, 1)
 compact_plan_kernel(const PoolParams p, CompactScratch ws, CompactOut out) {
   __shared__ int s_warp[32];
-  pdl_launch_dependents();
-  pdl_wait_primary();
+  pdl_enter();
   const int tid = threadIdx.x;
   const int lane = tid & 31;
   const int64_t first = int64_t(tid >> 5) * 32 * kScanRows + lane;
@@ -360,8 +356,7 @@ compact_plan_kernel(const PoolParams p, CompactScratch ws, CompactOut out) {
 
 template <bool kVec>
 __global__ void __launch_bounds__(kCopyThreads) compact_apply_kernel(const PoolParams p, CompactScratch ws, CompactOut out) {
-  pdl_launch_dependents();
-  pdl_wait_primary();
+  pdl_enter();
   const int cap = p.table_stride * kBlockTokens;
   const int moves = ws.moves[0];
   // Rows read remap while moving blocks' entries go from a place in the list to the id it stands for:
@@ -490,6 +485,7 @@ int aeg_fork_blocks(void* pool, size_t block_bytes, int64_t num_blocks, int32_t*
   AEG_CHECK_CUDA(aeg::launch(aeg::vectors(p) ? aeg::fork_apply_kernel<true> : aeg::fork_apply_kernel<false>, grid,
                              aeg::kCopyThreads, s, p, static_cast<int>(n), ws));
   AEG_CHECK_LAUNCH("fork_blocks");
+  aeg::note_launch(s, false);
   return AEG_OK;
 }
 
@@ -504,6 +500,7 @@ int aeg_free_blocks(int64_t num_blocks, int32_t* ref_counts, const int32_t* bloc
   AEG_CHECK_ARG(d_rows != nullptr && aeg::aligned(d_rows, 8), "free_blocks: null or misaligned row array");
   AEG_CHECK_CUDA(aeg::launch(aeg::free_kernel, n, aeg::kCopyThreads, static_cast<cudaStream_t>(stream), p, d_rows));
   AEG_CHECK_LAUNCH("free_blocks");
+  aeg::note_launch(static_cast<cudaStream_t>(stream), false);
   return AEG_OK;
 }
 
@@ -540,6 +537,7 @@ int aeg_compact_blocks(void* pool, size_t block_bytes, int64_t num_blocks, const
   AEG_CHECK_CUDA(aeg::launch(aeg::vectors(p) ? aeg::compact_apply_kernel<true> : aeg::compact_apply_kernel<false>, grid,
                              aeg::kCopyThreads, s, p, ws, out));
   AEG_CHECK_LAUNCH("compact_blocks");
+  aeg::note_launch(s, false);
   return AEG_OK;
 }
 

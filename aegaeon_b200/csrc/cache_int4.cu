@@ -61,13 +61,13 @@ struct Rows {
   int64_t num_slots;
   int64_t tokens;
   int heads;
+  bool early;  // of a write: let the next kernel launch before the wait
 };
 
 template <typename T, bool kVec, int kTokens, int kHeads>
 __global__ void __launch_bounds__(kThreads) write_int4_kernel(const Rows p) {
   constexpr int kItems = kTokens * kHeads;
-  pdl_launch_dependents();
-  pdl_wait_primary();
+  pdl_enter_write(p.early);
   const int lane = threadIdx.x & 31, l = lane & 15;
   const bool is_key = lane < 16;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWarpsPerCta * kTokens;
@@ -128,8 +128,7 @@ __global__ void __launch_bounds__(kThreads) write_int4_kernel(const Rows p) {
 template <typename T, bool kVec, int kTokens, int kHeads>
 __global__ void __launch_bounds__(kThreads) gather_int4_kernel(const Rows p) {
   constexpr int kItems = kTokens * kHeads;
-  pdl_launch_dependents();
-  pdl_wait_primary();
+  pdl_enter();
   const int lane = threadIdx.x & 31, l = lane & 15;
   const bool is_key = lane < 16;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWarpsPerCta * kTokens;
@@ -224,7 +223,7 @@ Kernel pick(bool write, bool vec, int64_t items, int heads, int* tokens, int* ch
   return heads == 1 ? pick<T, 4, 1>(write, vec) : pick<T, 2, 2>(write, vec);
 }
 
-int launch(const char* what, bool write, const Rows& p, int dtype, cudaStream_t stream) {
+int launch(const char* what, bool write, Rows& p, int dtype, cudaStream_t stream) {
   const bool vec = aligned(p.key, 16) && aligned(p.value, 16) && p.key_stride % 8 == 0 && p.value_stride % 8 == 0;
   int tokens = 1, chunk = 1;
   const Kernel k = dtype == AEG_DTYPE_BF16 ? pick<__nv_bfloat16>(write, vec, p.tokens * p.heads, p.heads, &tokens, &chunk)
@@ -243,8 +242,10 @@ int launch(const char* what, bool write, const Rows& p, int dtype, cudaStream_t 
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  p.early = write && follows_attention(stream);
   AEG_CHECK_CUDA(cudaLaunchKernelEx(&cfg, k, p));
   AEG_CHECK_LAUNCH(what);
+  note_launch(stream, false);
   return AEG_OK;
 }
 

@@ -23,13 +23,15 @@ constexpr int kCacheThreads = 128;
 constexpr int kWarpKernelThreads = 256;
 constexpr int64_t kWarpKernelMinTokens = 1024;  // from this many tokens on, one warp per token
 
-// The kernels run under programmatic dependent launch. Each first lets the next kernel launch
-// and then waits for the preceding one (which may have produced the keys, values or slots)
-// before reading anything: the next kernel's CTAs can then take SMs as the preceding kernel's
+// The kernels run under programmatic dependent launch: each waits for the preceding kernel (which
+// may have produced the keys, values or slots) before reading anything. Directly behind a decode
+// attention each first lets the next kernel launch: its CTAs can then take SMs as the attention's
 // leave, as they would if this launch were not between them (the decode attention after it
 // requests its first tiles early and waits for this kernel before reading a row it writes; a
 // kernel launched after it reads its results only after its own grid-dependency wait, which
-// covers this kernel, and this kernel completes only after the one before it). Measured on the
+// covers this kernel, and this kernel completes only after the one before it). Behind any other
+// kernel that could be another write, which an early start must not pass: the next kernel
+// launches after the wait then. Measured on the
 // reference's two-call layer (cache write, then attention): a cfg2 step 1.14 x the fused one
 // instead of 1.25 x, cfg3 1.02 x instead of 1.07 x. Each thread issues its first row loads
 // together with the slot load, so a token costs one global round trip before its stores.
@@ -37,9 +39,8 @@ __global__ void __launch_bounds__(kCacheThreads)
 reshape_and_cache_vec_kernel(const uint4* __restrict__ key, const uint4* __restrict__ value, int64_t key_stride_v,
                              int64_t value_stride_v, uint4* __restrict__ k_cache, uint4* __restrict__ v_cache,
                              int64_t block_stride_v, int64_t num_slots, const int64_t* __restrict__ slot_mapping,
-                             int row_vecs) {
-  pdl_launch_dependents();
-  pdl_wait_primary();
+                             int row_vecs, bool early) {
+  pdl_enter_write(early);
   const int64_t t = blockIdx.x;
   const int i0 = threadIdx.x;
   uint4 first = make_uint4(0u, 0u, 0u, 0u);
@@ -72,9 +73,8 @@ __global__ void __launch_bounds__(kWarpKernelThreads)
 reshape_and_cache_warp_kernel(const uint4* __restrict__ key, const uint4* __restrict__ value, int64_t key_stride_v,
                               int64_t value_stride_v, uint4* __restrict__ k_cache, uint4* __restrict__ v_cache,
                               int64_t block_stride_v, int64_t num_slots, const int64_t* __restrict__ slot_mapping,
-                              int row_vecs, int64_t T) {
-  pdl_launch_dependents();
-  pdl_wait_primary();
+                              int row_vecs, int64_t T, bool early) {
+  pdl_enter_write(early);
   const int lane = threadIdx.x & 31;
   const int64_t warps = static_cast<int64_t>(gridDim.x) * (kWarpKernelThreads / 32);
   for (int64_t t = (static_cast<int64_t>(blockIdx.x) * kWarpKernelThreads + threadIdx.x) >> 5; t < T; t += warps) {
@@ -111,9 +111,8 @@ __global__ void __launch_bounds__(kCacheThreads)
 reshape_and_cache_elem_kernel(const uint16_t* __restrict__ key, const uint16_t* __restrict__ value,
                               int64_t key_stride, int64_t value_stride, uint16_t* __restrict__ k_cache,
                               uint16_t* __restrict__ v_cache, int64_t block_stride, int64_t num_slots,
-                              const int64_t* __restrict__ slot_mapping, int row_elems) {
-  pdl_launch_dependents();
-  pdl_wait_primary();
+                              const int64_t* __restrict__ slot_mapping, int row_elems, bool early) {
+  pdl_enter_write(early);
   const int64_t t = blockIdx.x;
   const int64_t slot = slot_mapping[t];
   if (slot < 0) return;
@@ -169,6 +168,7 @@ extern "C" int aeg_reshape_and_cache(const void* key, const void* value, int64_t
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  const bool early = aeg::follows_attention(s);
   if (vec && T >= aeg::kWarpKernelMinTokens) {
     int dev = 0, sms = 0;
     AEG_CHECK_CUDA(cudaGetDevice(&dev));
@@ -179,18 +179,19 @@ extern "C" int aeg_reshape_and_cache(const void* key, const void* value, int64_t
     AEG_CHECK_CUDA(cudaLaunchKernelEx(&cfg, aeg::reshape_and_cache_warp_kernel, static_cast<const uint4*>(key),
                                       static_cast<const uint4*>(value), key_stride / 8, value_stride / 8,
                                       static_cast<uint4*>(k_cache), static_cast<uint4*>(v_cache), block_stride / 8,
-                                      num_slots, slot_mapping, static_cast<int>(row / 8), T));
+                                      num_slots, slot_mapping, static_cast<int>(row / 8), T, early));
   } else if (vec) {
     AEG_CHECK_CUDA(cudaLaunchKernelEx(&cfg, aeg::reshape_and_cache_vec_kernel, static_cast<const uint4*>(key),
                                       static_cast<const uint4*>(value), key_stride / 8, value_stride / 8,
                                       static_cast<uint4*>(k_cache), static_cast<uint4*>(v_cache), block_stride / 8,
-                                      num_slots, slot_mapping, static_cast<int>(row / 8)));
+                                      num_slots, slot_mapping, static_cast<int>(row / 8), early));
   } else {
     AEG_CHECK_CUDA(cudaLaunchKernelEx(&cfg, aeg::reshape_and_cache_elem_kernel, static_cast<const uint16_t*>(key),
                                       static_cast<const uint16_t*>(value), key_stride, value_stride,
                                       static_cast<uint16_t*>(k_cache), static_cast<uint16_t*>(v_cache), block_stride,
-                                      num_slots, slot_mapping, static_cast<int>(row)));
+                                      num_slots, slot_mapping, static_cast<int>(row), early));
   }
   AEG_CHECK_LAUNCH("reshape_and_cache");
+  aeg::note_launch(s, false);
   return AEG_OK;
 }

@@ -1825,7 +1825,10 @@ int decode_launch(const DecodeLaunch& dl, cudaStream_t s, LaunchOrder& order) {
                     : launch_attn_t<__nv_bfloat16, 2>(dl.km, dl.vm, dl.prm, s, ev);
   else
     st = dl.nt == 1 ? launch_attn_t<__half, 1>(dl.km, dl.vm, dl.prm, s, ev) : launch_attn_t<__half, 2>(dl.km, dl.vm, dl.prm, s, ev);
-  if (st == AEG_OK) order.launched();
+  if (st == AEG_OK) {
+    order.launched();
+    note_launch(s, !dl.prm.fuse_write);
+  }
   return st;
 }
 
@@ -1910,7 +1913,10 @@ int decode_int4(void* out, int64_t out_stride, const void* q, int64_t q_stride, 
   cudaEvent_t ev = order.event();
   st = bf ? (one ? launch_attn_int4<__nv_bfloat16, 1>(prm, s, ev) : launch_attn_int4<__nv_bfloat16, 2>(prm, s, ev))
           : (one ? launch_attn_int4<__half, 1>(prm, s, ev) : launch_attn_int4<__half, 2>(prm, s, ev));
-  if (st == AEG_OK) order.launched();
+  if (st == AEG_OK) {
+    order.launched();
+    note_launch(s, true);
+  }
   return st;
 }
 

@@ -81,8 +81,7 @@ template <typename T, int kVec>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) {
   using V = typename Vec<kVec>::Type;
   __shared__ float s_cos[2][kMaxHalf], s_sin[2][kMaxHalf];
-  pdl_launch_dependents();
-  pdl_wait_primary();
+  pdl_enter();
   const int tid = threadIdx.x;
   const int per_head = p.half / kVec;            // rotated vectors of a head (each with its partner)
   const int rest = p.dim / kVec - 2 * per_head;  // copied vectors of a head
@@ -230,5 +229,6 @@ extern "C" int aeg_rotary_multi_axis(void* q_out, int64_t q_out_stride, void* k_
   cfg.numAttrs = 1;
   AEG_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
   AEG_CHECK_LAUNCH("rotary_multi_axis");
+  aeg::note_launch(cfg.stream, false);
   return AEG_OK;
 }

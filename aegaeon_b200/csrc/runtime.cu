@@ -2,6 +2,7 @@
 // sticky device error word reader.
 #include "aeg_common.cuh"
 
+#include <atomic>
 #include <mutex>
 #include <vector>
 
@@ -34,6 +35,38 @@ int num_sms() {
     cache[dev] = n;
   }
   return cache[dev];
+}
+
+// Per device the stream whose last noted launch is an attention; one at a time, so that another stream's
+// attention makes this one's writes start their successors later, never sooner.
+namespace {
+constexpr int kTailDevices = 64;
+struct Tail {
+  std::atomic<bool> any{false};
+  std::atomic<cudaStream_t> stream{nullptr};
+};
+Tail* tail() {
+  static Tail t[kTailDevices];
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kTailDevices ? &t[dev] : nullptr;
+}
+}  // namespace
+
+bool follows_attention(cudaStream_t s) {
+  const Tail* t = tail();
+  return t != nullptr && t->any.load() && t->stream.load() == s;
+}
+
+void note_launch(cudaStream_t s, bool attention) {
+  Tail* t = tail();
+  if (t == nullptr) return;
+  if (attention) {
+    t->any.store(false);  // no moment in which another stream passes for this one
+    t->stream.store(s);
+    t->any.store(true);
+  } else if (t->stream.load() == s) {
+    t->any.store(false);
+  }
 }
 
 }  // namespace aeg

@@ -303,7 +303,10 @@ AEG_API int aeg_decode_plan(void* workspace, size_t workspace_bytes, const int32
  * `stream`, so the launch may request its first K/V tiles before that kernel has finished (the
  * query rows and new K/V rows are still read only after it). Safe between consecutive layers of
  * one decode step (a layer writes only its own layer's rows); not after a cache write, a block
- * copy or a swap of the same layer.
+ * copy or a swap of the same layer. The kernels of this library that lie between may not be passed
+ * further than that: each starts its successor only after its own wait, a cache write sooner only
+ * behind an unfused decode attention. A kernel of another library that lets its successor start
+ * before its own grid-dependency wait counts together with the kernel before it.
  * AEG_DECODE_PREFETCH_AFTER_DECODE_WRITE (aeg_paged_attn_decode): the kernel that immediately
  * precedes the call wrote, of what the call reads, at most position seq_lens[b] - 1 of each
  * sequence (the decode cache write of aeg_reshape_and_cache with the slots the reference builds
