@@ -347,7 +347,7 @@ template <typename T, int NT>
 __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_kernel(const AttnParams p) {
   using SL = Int4Smem<NT>;
   constexpr int kW = SL::kWarps, kSt = SL::kStages;
-  constexpr float kNoMax = -1e30f;  // the running maximum before the first score
+  constexpr float kNoMax = -3e38f;  // the running maximum before the first score, below all but infinite ones
   constexpr float kSlack = 6.f;     // scores may exceed the running maximum by this (log2 units)
   constexpr float kTop = 512.f;     // largest scaled scale: 2^9 * 2^kSlack = 2^15 fits fp16
   constexpr int kFold = 16;         // tiles between two removals of the constant from O
@@ -523,11 +523,11 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
     }
     first = false;
 
-    // Running maximum of the unscaled scores, that times the scale, and the score from which it moves;
-    // sum of p; sum of p * (minimum + middle * scale) [column][group]; sum of the rounded P * scale
-    // [group]. O and the last are held times `vmul`.
+    // Running maximum of the unscaled scores and the score from which it moves (rounded down: p stays
+    // within 2^kSlack however coarse the scores are); sum of p; sum of p * (minimum + middle * scale)
+    // [column][group]; sum of the rounded P * scale [group]. O and the last are held times `vmul`.
     float o[8][NT][4];
-    float m[NT][2], ms[NT][2], mt_[NT][2], l[NT][2], om[NT][2][2], ps[2][NT][4];
+    float m[NT][2], mt_[NT][2], l[NT][2], om[NT][2][2], ps[2][NT][4];
     float vmul = kTop;
     uint32_t vlim = 0;  // bits of the largest scale allowed for
 #pragma unroll
@@ -535,8 +535,7 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         m[nt][i] = kNoMax;
-        ms[nt][i] = kNoMax * sc[nt][i];
-        mt_[nt][i] = kNoMax + kSlack / sc[nt][i];
+        mt_[nt][i] = __fadd_rd(kNoMax, kSlack / sc[nt][i]);
         l[nt][i] = om[nt][i][0] = om[nt][i][1] = 0.f;
         ps[i][nt][0] = ps[i][nt][1] = ps[i][nt][2] = ps[i][nt][3] = 0.f;
       }
@@ -624,8 +623,7 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
           for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
           const float mn = fmaxf(m[nt][i], mx), a = ex2((m[nt][i] - mn) * sc[nt][i]);
           m[nt][i] = mn;
-          ms[nt][i] = mn * sc[nt][i];
-          mt_[nt][i] = mn + kSlack / sc[nt][i];
+          mt_[nt][i] = __fadd_rd(mn, kSlack / sc[nt][i]);
           l[nt][i] *= a;
           om[nt][i][0] *= a;
           om[nt][i][1] *= a;
@@ -670,7 +668,8 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
       const uint8_t* vcodes = tile + kInt4ValueCodes + quad * 128 + grp * 16;
       const uint4 vc0 = lds128(vcodes), vc1 = lds128(vcodes + 512);
 
-      // P, its sums, and P * scale of each group, turned around in registers.
+      // P, its sums, and P * scale of each group, turned around in registers. The maximum is taken off before
+      // the product with the scale: of the largest score exactly 0 remains, whatever its size.
       uint32_t pv[2][NT][2];
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
@@ -682,7 +681,7 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
           float* p_ = x[nt];
           if (g == 0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p_[i] = ex2(fmaf(p_[i], sc[nt][i & 1], -ms[nt][i & 1]));
+            for (int i = 0; i < 4; ++i) p_[i] = ex2((p_[i] - m[nt][i & 1]) * sc[nt][i & 1]);
             l[nt][0] += p_[0] + p_[2];
             l[nt][1] += p_[1] + p_[3];
           }
@@ -773,7 +772,8 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
             po[1] = make_float4(y[4], y[5], y[6], y[7]);
           }
         }
-        if (slot >= 0 && grp == 0) p.ws.part_ml[static_cast<int64_t>(slot) * G + head] = make_float2(ms[nt][i], l[nt][i]);
+        if (slot >= 0 && grp == 0)  // a finite maximum of a piece without tokens too
+          p.ws.part_ml[static_cast<int64_t>(slot) * G + head] = make_float2(fmaxf(m[nt][i] * sc[nt][i], kNoMax), l[nt][i]);
       }
   }
 

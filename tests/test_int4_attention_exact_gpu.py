@@ -1,5 +1,5 @@
 """Decode attention over a 4-bit cache whose values lie far apart, against the oracle in 64 bits: poisoned groups
-beside finite ones."""
+beside finite ones, and scores too large for a difference of rounded products."""
 import pytest
 import torch
 
@@ -45,3 +45,27 @@ def test_a_poisoned_group_leaves_the_other_group_alone(cuda_device, dtype, size,
     pairs[block, 0, 1::4, 1, 0, 1] = float("nan")  # dims 64..127
     tables = torch.arange(19, dtype=torch.int32).repeat(3, 1).numpy()
     _check(cuda_device, _q(dtype, 3, Hkv), cache, tables, lens, _bound)
+
+
+@BOTH
+@pytest.mark.parametrize("size,sign", [(2.0 ** 10, 1), (2.0 ** 14, 1), (2.0 ** 14, -1), (1e17, 1), (1e17, -1)])
+def test_scores_of_any_size_pick_the_largest(cuda_device, dtype, size, sign):
+    """Queries and keys that are constant over their dims: scores of +-2^24 to 2^120 in log2 units, the largest
+    ahead of the others by 10^6 and more. The output is that token's value row."""
+    if size > 65504 and dtype == torch.float16:
+        size = 2.0 ** 15
+    for n in (3, 90, 250):
+        cache = _cache(dtype, 16, 1, 2, n)
+        pairs = _pairs(cache)
+        best = n // 2
+        steps = torch.randperm(256, generator=torch.Generator().manual_seed(n)) % 100
+        steps[best] = 200
+        unit = size * torch.finfo(dtype).eps if dtype == torch.float16 else size / 1024  # bf16: all but the best round alike
+        pairs[:, 0, :, 0, :, :, 0] = 0
+        pairs[:, 0, :, 0, :, :, 1] = (sign * (size + sign * unit * steps.float())).to(dtype).view(16, 1, 16, 1)
+        q = torch.full((1, 8, 128), size, dtype=dtype)
+        got = _run(cuda_device, q, cache, 0, torch.arange(16, dtype=torch.int32).view(1, 16).numpy(), [n])
+        want = ref.values(cache[:, 0])[1][best // 16, :, best % 16].repeat_interleave(4, 0)
+        # P * s with 11 bits times codes up to 8 off the middle; the scale is below 0.35, the minimum below 8
+        bound = want.abs() * torch.finfo(dtype).eps / 2 + 2.0 ** -11 * 8 * 0.35 + 2.0 ** -20 * 8
+        assert ((got[0].double() - want).abs() <= bound).all()
