@@ -8,22 +8,22 @@
 //       q . K = sum over groups of  s (q . c) + m (sum of q)
 //       sum_t p_t V_t = sum_t (p_t s_t) c_t + sum_t p_t m_t
 //     so the codes go to the tensor cores as they are, exactly, and scales and minima meet them
-//     in fp32. A code becomes an fp16 number with one AND-OR: a nibble under the exponent of 64 reads
-//     as 64 + c, and the constant is taken out with the keys' minima (m - 64 s in place of m) in fp32;
-//     of the values, see the fold below.
+//     in fp32. A key code becomes an fp16 number with one AND-OR: a nibble under the exponent of 64 reads
+//     as 64 + c, and the constant is taken out with the keys' minima (m - 64 s in place of m) in fp32.
 //   * S^T = K Q^T as in the 16-bit kernel (16 tokens x 8 heads of the group, m16n8k16), in fp16 for bf16
 //     queries too, scaled by a power of two. A lane's codes of a token are one 16-byte load; which dim
 //     sits where in the contraction is free as long as the query fragments follow.
-//   * O^T += V^T P^T with codes and P * s as fp16, P * s brought to within 2^15 by a power of two that
-//     follows the largest scale the warp has met: 11 bits for everything down to 2^-23 of the
-//     largest product (bf16 would keep 8 and need a second MMA for the rest). Token pairs share a
-//     32-bit word, so that the transposed fragment comes out of the same AND-OR without a
-//     transposing load. sum p m is 4 FMAs a token and lane.
-//   * The constant multiplies the rounded P * s, so its share is summed from those (one more MMA a
-//     group, with ones) and cancels exactly; what remains is sum (P s)(c - 8) and, in fp32, sum p (m + 8 s).
-//     The tensor cores cut off what an addition pushes out of the accumulator, always downwards, so a sum
-//     that carries the constant along drifts with its length (128 sum(p s) over 4096 tokens: 2.5 times
-//     the error of the output's own rounding). So it is taken out of O every kFold tiles.
+//   * O^T += V^T P^T in bf16: P * s, made in fp32, goes in as two bf16 parts (16 bits), each with the whole
+//     range of fp32's exponents, so that neither a token's nor a group's scale costs another one bits. A
+//     value code becomes a bf16 number with one AND: a nibble under a zero exponent is the subnormal
+//     c * 2^-133, or c * 2^-129 four bits further up (bf16's least normal binade has the spacing of its
+//     subnormals), exact on the tensor cores. P * s is held times a power of two that keeps the products
+//     away from fp32's ends. Token pairs share a 32-bit word, so that the transposed fragment comes out of
+//     the AND without a transposing load. sum p m is 4 FMAs a token and lane.
+//   * The tensor cores cut off what an addition pushes out of the accumulator, always downwards, so a sum
+//     of one sign drifts with its length. So odd tokens count from the top: with -P s they meet 15 - c (the
+//     AND's result with those four bits turned over, the same instruction), sum p (m + 15 s) in place of
+//     their sum p m makes up for it, and O stays near 0.
 //   * The running maximum moves only when a score exceeds it by kSlack (log2 units): sums are fp32, and
 //     most tiles need one vote instead of a reduction over the tokens and a rescaling of O.
 //   * One warp of the CTA requests the tiles of all others, a lane for each, so that walking the units
@@ -89,23 +89,42 @@ __device__ __forceinline__ void code_pairs(uint32_t w, uint32_t (&a)[4]) {
   a[2] = up(and_or(t, 0x000f000fu, 0x54005400u));
   a[3] = and_or(t, 0x00f000f0u, 0x54005400u);
 }
-// Values count from the middle code, which keeps the sums of rounded P * scale small.
-constexpr float kMiddle = 8.f;
-// Bits of a scale: infinity, and the mantissa.
-template <typename T>
-constexpr uint32_t kScaleInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-template <typename T>
-constexpr float kScaleLeast = std::is_same<T, __half>::value ? 0x1p-14f : 0x1p-100f;  // smaller ones count as this
-template <typename T>
-constexpr uint32_t kScaleMantissa = std::is_same<T, __half>::value ? 0x3ffu : 0x7fu;
+// The same nibbles of a value word as bf16 pairs: a[0], a[2] hold code * 2^-133, a[1], a[3] code * 2^-129, the
+// upper halves, which are odd tokens, 15 - code.
+__device__ __forceinline__ void value_codes(uint32_t w, uint32_t (&a)[4]) {
+  const uint32_t t = w >> 8;
+  a[0] = (w & 0x000f000fu) ^ 0x000f0000u;
+  a[1] = (w & 0x00f000f0u) ^ 0x00f00000u;
+  a[2] = (t & 0x000f000fu) ^ 0x000f0000u;
+  a[3] = (t & 0x00f000f0u) ^ 0x00f00000u;
+}
+// Two fp32 numbers as pairs of bf16: the upper 8 bits of each cut off, and the rest rounded to 8.
+__device__ __forceinline__ void split2(float y0, float y1, uint32_t& hi, uint32_t& lo) {
+  const uint32_t b0 = __float_as_uint(y0), b1 = __float_as_uint(y1);
+  hi = __byte_perm(b0, b1, 0x7632);
+  lo = pack2<__nv_bfloat16>(y0 - __uint_as_float(b0 & 0xffff0000u), y1 - __uint_as_float(b1 & 0xffff0000u));
+}
+// What P * scale is held times. fp16's scales, 2^-24 to 2^13, go with this one number; over bf16's range it
+// follows the largest finite scale met, which it brings to 2^96 or up to 2^17 times that (2^127 is its own end).
+// Products and sums then stay below 2^11, and the 16 bits of a scale 2^-96 of the largest above fp32's last.
+constexpr float kTop = 0x1p96f;
+constexpr uint32_t kScaleInf = 0x7f80u;   // bits of a bf16 infinity
+constexpr float kScaleLeast = 0x1p-31f;   // smaller scales count as this
+constexpr uint32_t kScaleRoom = 0x087fu;  // added to a scale's exponent: the largest one with the same factor
 
 // Products, transpositions and shared loads that the compiler may move among one another (those of
 // aeg_common.cuh are volatile and keep their order): a tile's chains overlap only if it does. The
 // loads stay behind the barrier waits, which clobber memory.
+template <typename T>
 __device__ __forceinline__ void mma_free(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose_free(uint32_t a) {
   uint32_t d;
@@ -349,9 +368,6 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
   constexpr int kW = SL::kWarps, kSt = SL::kStages;
   constexpr float kNoMax = -3e38f;  // the running maximum before the first score, below all but infinite ones
   constexpr float kSlack = 6.f;     // scores may exceed the running maximum by this (log2 units)
-  constexpr float kTop = 512.f;     // largest scaled scale: 2^9 * 2^kSlack = 2^15 fits fp16
-  constexpr int kFold = 16;         // tiles between two removals of the constant from O
-  const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -524,12 +540,14 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
     first = false;
 
     // Running maximum of the unscaled scores and the score from which it moves (rounded down: p stays
-    // within 2^kSlack however coarse the scores are); sum of p; sum of p * (minimum + middle * scale)
-    // [column][group]; sum of the rounded P * scale [group]. O and the last are held times `vmul`.
+    // within 2^kSlack however coarse the scores are); sum of p; sum of p * (what code 0 stands for)
+    // [column][group]. O is held times |vmul|, which has the sign of this lane's tokens.
     float o[8][NT][4];
-    float m[NT][2], mt_[NT][2], l[NT][2], om[NT][2][2], ps[2][NT][4];
-    float vmul = kTop;
-    uint32_t vlim = 0;  // bits of the largest scale allowed for
+    float m[NT][2], mt_[NT][2], l[NT][2], om[NT][2][2];
+    const bool odd = grp & 1;
+    const float code0 = odd ? 15.f : 0.f;
+    float vmul = odd ? -kTop : kTop;
+    uint32_t vlim = 0;  // bits of the largest scale allowed for (bf16)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -537,25 +555,10 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
         m[nt][i] = kNoMax;
         mt_[nt][i] = __fadd_rd(kNoMax, kSlack / sc[nt][i]);
         l[nt][i] = om[nt][i][0] = om[nt][i][1] = 0.f;
-        ps[i][nt][0] = ps[i][nt][1] = ps[i][nt][2] = ps[i][nt][3] = 0.f;
       }
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt) o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.f;
     }
-    // Takes the codes' constant out of O.
-    auto fold = [&]() {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-#pragma unroll
-          for (int mt = 4 * g; mt < 4 * g + 4; ++mt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[mt][nt][i] = fmaf(-(kBias + kMiddle), ps[g][nt][i], o[mt][nt][i]);
-          ps[g][nt][0] = ps[g][nt][1] = ps[g][nt][2] = ps[g][nt][3] = 0.f;
-        }
-    };
-
     // Scores of the tile in stage `st`, unscaled: S^T, one accumulator per group; rows are tokens grp
     // and grp + 8.
     auto scores = [&](uint32_t st, float (*x)[4]) {
@@ -577,7 +580,7 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
           for (int u = 0; u < 2; ++u) {
             const uint32_t a[4] = {lo[2 * u], hi[2 * u], lo[2 * u + 1], hi[2 * u + 1]};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_free(s[nt], a, qf[nt][2 * w + u][0], qf[nt][2 * w + u][1]);
+            for (int nt = 0; nt < NT; ++nt) mma_free<__half>(s[nt], a, qf[nt][2 * w + u][0], qf[nt][2 * w + u][1]);
           }
         }
         const float2 f0 = unpack2<T>(g == 0 ? kp0.x : kp0.y), f1 = unpack2<T>(g == 0 ? kp1.x : kp1.y);
@@ -595,24 +598,25 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
     // Makes room for the scores x and the scales of the value pairs vp0, vp1: the maxima move to the tile's,
     // and what was summed so far follows.
     auto make_room = [&](const float (*x)[4], const uint2& vp0, const uint2& vp1) {
-      // Of the finite scales alone: NaN needs no room, it makes its own group's result NaN by itself, and the
-      // other group of the head goes on.
-      uint32_t top = 0;
-      for (const uint32_t pair : {vp0.x, vp0.y, vp1.x, vp1.y}) {
-        const uint32_t scale = pair & 0xffffu;
-        if (scale < kScaleInf<T>) top = max(top, scale);
-      }
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
       float grow = 1.f;
-      if (top > vlim) {
-        // The power of two above the scale, kept in range for the tiniest ones.
-        const float t = fmaxf(unpack2<T>(top).x, kScaleLeast<T>);
-        const uint32_t e = __float_as_uint(t) >> 23;  // t in [2^(e - 127), 2^(e - 126))
-        const float next = __uint_as_float((253u - e) << 23) * kTop;
-        grow = next / vmul;
-        vmul = next;
-        vlim = bits16(from_float<T>(t)) | kScaleMantissa<T>;
+      if constexpr (!std::is_same<T, __half>::value) {
+        // Of the finite scales alone: NaN needs no room, it makes its own group's result NaN by itself, and
+        // the other group of the head goes on.
+        uint32_t top = 0;
+        for (const uint32_t pair : {vp0.x, vp0.y, vp1.x, vp1.y}) {
+          const uint32_t scale = pair & 0xffffu;
+          if (scale < kScaleInf) top = max(top, scale);
+        }
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+        if (top > vlim) {
+          const uint32_t bits = max(top << 16, __float_as_uint(kScaleLeast));
+          const uint32_t e = bits >> 23;  // the scale lies in [2^(e - 127), 2^(e - 126))
+          const float next = copysignf(__uint_as_float((254u + 96u - e) << 23), vmul);  // 2^96 / 2^(e - 127)
+          grow = next / vmul;
+          vmul = next;
+          vlim = min((e << 7) + kScaleRoom, kScaleInf - 1);
+        }
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -628,10 +632,6 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
           om[nt][i][0] *= a;
           om[nt][i][1] *= a;
           const float ao = a * grow;
-          ps[0][nt][i] *= ao;
-          ps[0][nt][i + 2] *= ao;
-          ps[1][nt][i] *= ao;
-          ps[1][nt][i + 2] *= ao;
 #pragma unroll
           for (int mt = 0; mt < 8; ++mt) {
             o[mt][nt][i] *= ao;
@@ -656,9 +656,9 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
         if (!in0) vp0 = make_uint2(0u, 0u);
         if (!in1) vp1 = make_uint2(0u, 0u);
       }
-      // Scales are not negative, so their bits are in their order; NaN is above all.
-      const uint32_t vtop = __vmaxu2(__vmaxu2(vp0.x, vp0.y), __vmaxu2(vp1.x, vp1.y)) & 0xffffu;
-      bool over = vtop > vlim;
+      bool over = false;
+      if constexpr (!std::is_same<T, __half>::value)  // scales are not negative: their bits are in their order, NaN above all
+        over = (__vmaxu2(__vmaxu2(vp0.x, vp0.y), __vmaxu2(vp1.x, vp1.y)) & 0xffffu) > vlim;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -670,11 +670,11 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
 
       // P, its sums, and P * scale of each group, turned around in registers. The maximum is taken off before
       // the product with the scale: of the largest score exactly 0 remains, whatever its size.
-      uint32_t pv[2][NT][2];
+      uint32_t pv[2][NT][2][2];  // [group][column tile][tokens 0..7, 8..15][part]
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const float2 f0 = unpack2<T>(g == 0 ? vp0.x : vp0.y), f1 = unpack2<T>(g == 0 ? vp1.x : vp1.y);
-        const float b0 = fmaf(kMiddle, f0.x, f0.y), b1 = fmaf(kMiddle, f1.x, f1.y);
+        const float b0 = fmaf(code0, f0.x, f0.y), b1 = fmaf(code0, f1.x, f1.y);
         const float s0 = f0.x * vmul, s1 = f1.x * vmul;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -687,9 +687,13 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
           }
           om[nt][0][g] = fmaf(p_[0], b0, fmaf(p_[2], b1, om[nt][0][g]));
           om[nt][1][g] = fmaf(p_[1], b0, fmaf(p_[3], b1, om[nt][1][g]));
-          pv[g][nt][0] = transpose_free(pack2<__half>(p_[0] * s0, p_[1] * s0));
-          pv[g][nt][1] = transpose_free(pack2<__half>(p_[2] * s1, p_[3] * s1));
-          mma_free(ps[g][nt], ones, pv[g][nt][0], pv[g][nt][1]);
+          split2(p_[0] * s0, p_[1] * s0, pv[g][nt][0][0], pv[g][nt][0][1]);
+          split2(p_[2] * s1, p_[3] * s1, pv[g][nt][1][0], pv[g][nt][1][1]);
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            pv[g][nt][0][part] = transpose_free(pv[g][nt][0][part]);
+            pv[g][nt][1][part] = transpose_free(pv[g][nt][1][part]);
+          }
         }
       }
 
@@ -698,13 +702,16 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         uint32_t lo[4], hi[4];
-        code_pairs(vw0[w], lo);
-        code_pairs(vw1[w], hi);
+        value_codes(vw0[w], lo);
+        value_codes(vw1[w], hi);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t a[4] = {lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1]};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_free(o[2 * w + j][nt], a, pv[w >> 1][nt][0], pv[w >> 1][nt][1]);
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int part = 0; part < 2; ++part)
+              mma_free<__nv_bfloat16>(o[2 * w + j][nt], a, pv[w >> 1][nt][0][part], pv[w >> 1][nt][1][part]);
         }
       }
     };
@@ -715,7 +722,6 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
       if (lost) break;
       scores(st_con, x);
       add_tile(st_con, x);
-      if ((k & (kFold - 1)) == kFold - 1) fold();
       // Every lane's reads of the stage have fed its products.
       __syncwarp();
       if (lane == 0) mbar_arrive(&wk.empty[st_con]);
@@ -737,8 +743,8 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
           om[nt][i][0] += __shfl_xor_sync(0xffffffffu, om[nt][i][0], off);
           om[nt][i][1] += __shfl_xor_sync(0xffffffffu, om[nt][i][1], off);
         }
-    fold();
-    const float unit_o = __uint_as_float((254u << 23) - __float_as_uint(vmul));  // 1 / vmul, a power of two
+    // 2^63 / |vmul|; with 2^70 and 2^66 the units of the codes and that, in two steps within fp32's range.
+    const float unit_o = __uint_as_float((317u << 23) - __float_as_uint(fabsf(vmul)));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -750,8 +756,8 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
           float y[8];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            y[2 * j] = fmaf(o[4 * g + j][nt][i], unit_o, om[nt][i][g]);
-            y[2 * j + 1] = fmaf(o[4 * g + j][nt][i + 2], unit_o, om[nt][i][g]);
+            y[2 * j] = fmaf(o[4 * g + j][nt][i] * 0x1p70f, unit_o, om[nt][i][g]);
+            y[2 * j + 1] = fmaf(o[4 * g + j][nt][i + 2] * 0x1p66f, unit_o, om[nt][i][g]);
           }
           if (slot < 0) {
             const float inv = l[nt][i] == 0.f ? 0.f : __frcp_rn(l[nt][i]);

@@ -1,10 +1,22 @@
 """Decode attention over a 4-bit cache whose values lie far apart, against the oracle in 64 bits: poisoned groups
-beside finite ones, and scores too large for a difference of rounded products."""
+beside finite ones, scores too large for a difference of rounded products, tokens and groups whose scales differ
+by many powers of two.
+
+Tolerance (``_weighted``), from the exact weights w, scales s, minima m and values V of each token, for a
+sequence of n tokens (t tiles of 16):
+  * the output's own rounding: half a step of its value;
+  * w * s is kept to 16 bits, times codes of up to 15: 2^-16 * 15 * sum w s;
+  * two products a tile on the tensor cores, each cut off by up to 2^-22 of what the sum holds, at most
+    15 * sum w s: 2 t * 2^-22 of that; the sums of w m in fp32, (t + 8) * 2^-23 * sum w (|m| + 15 s);
+  * a score is off by 2^-22 for each of its 8 products and 8 more steps, of the sum of its absolute terms, A,
+    and by 2^-23 of itself in the exponent; a weight moves by twice that and by 2^-21 for its exponential and
+    the sum that divides it, the output by as much of sum w |V| and of itself."""
 import pytest
 import torch
 
 from aegaeon_b200 import ops
 from oracle import serving_ref as ref
+from tests.gpu_helpers import make_tables
 from tests.test_int4_attention_gpu import SCALE, _bound, _cache, _q, _run
 
 pytestmark = pytest.mark.gpu
@@ -16,6 +28,33 @@ def _pairs(cache):
     """(blocks, layers, heads, key/value, token, group, scale/minimum) of a CPU cache, a view."""
     N, L, Hkv, _ = cache.shape
     return cache[..., 1024:].view(N, L, Hkv, 2, 16, 2, 2)
+
+
+def _weighted(want, q, cache, layer, tables, lens, scale):
+    """The tolerance above, per output element. Keys' codes count with an offset of 64."""
+    B, Hq, _ = q.shape
+    Hkv = cache.size(2)
+    out = torch.empty_like(want)
+    for b in range(B):
+        n = int(lens[b])
+        tiles = (n + 15) // 16
+        ids = torch.as_tensor([int(i) for i in tables[b][:tiles]])
+        k, v = (x.transpose(0, 1).reshape(Hkv, -1, 128)[:, :n] for x in ref.values(cache[ids, 0]))
+        pairs = _pairs(cache)[ids, 0].double().permute(1, 2, 0, 3, 4, 5).reshape(Hkv, 2, -1, 2, 2)[:, :, :n]
+        qg = q[b].double().view(Hkv, -1, 128)
+        w = torch.softmax(torch.einsum("hgd,htd->hgt", qg, k) * scale, -1)
+        sk, mk = (pairs[:, 0, :, :, i].repeat_interleave(64, -1) for i in (0, 1))  # Hkv, n, 128
+        terms = torch.einsum("hgd,htd->hgt", qg.abs(), 2 * 79 * sk + mk.abs())  # 64 + c, and 64 s beside m
+        delta = (16 * 2.0 ** -22 + 2.0 ** -23) * terms.amax(-1) * abs(scale) * 1.5  # Hkv, G, in log2 units
+        sv, mv = (pairs[:, 1, :, :, i].repeat_interleave(64, -1).nan_to_num() for i in (0, 1))
+        ws = torch.einsum("hgt,htd->hgd", w, sv)
+        wm = torch.einsum("hgt,htd->hgd", w, mv.abs() + 15 * sv)
+        wv = torch.einsum("hgt,htd->hgd", w, v.abs().nan_to_num())
+        err = 15 * ws * (2.0 ** -16 + 2 * tiles * 2.0 ** -22) + wm * (tiles + 8) * 2.0 ** -23
+        err = err + (2 * delta.unsqueeze(-1) + 2.0 ** -21) * 2 * wv
+        out[b] = err.reshape(Hq, 128)
+    info = torch.finfo(q.dtype)
+    return out + want.abs() * info.eps / 2 + info.smallest_normal * info.eps
 
 
 def _check(dev, q, cache, tables, lens, bound):
@@ -69,3 +108,43 @@ def test_scores_of_any_size_pick_the_largest(cuda_device, dtype, size, sign):
         # P * s with 11 bits times codes up to 8 off the middle; the scale is below 0.35, the minimum below 8
         bound = want.abs() * torch.finfo(dtype).eps / 2 + 2.0 ** -11 * 8 * 0.35 + 2.0 ** -20 * 8
         assert ((got[0].double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype,large,small", [(torch.float16, 8000.0, 2.0 ** -12), (torch.bfloat16, 1e9, 0.3),
+                                               (torch.bfloat16, 1e20, 1e-3), (torch.bfloat16, 3.0, 1e-20)])
+def test_a_large_scale_without_weight_costs_the_others_nothing(cuda_device, dtype, large, small):
+    """One token's value scale is 2^24 times the others' and more, and no query looks at it."""
+    cache = _cache(dtype, 8, 1, 2, 6)
+    pairs = _pairs(cache)
+    g = torch.Generator().manual_seed(2)
+    pairs[..., 1, :, :, 0] = (small * (0.5 + torch.rand(8, 1, 2, 16, 2, generator=g))).to(dtype)
+    pairs[..., 1, :, :, 1] = (-7.5 * pairs[..., 1, :, :, 0].float()).to(dtype)
+    pairs[3, 0, :, 1, 5, :, 0] = large
+    pairs[3, 0, :, 1, 5, :, 1] = -7.5 * large
+    pairs[3, 0, :, 0, 5, :, 0] = 0.0
+    pairs[3, 0, :, 0, 5, :, 1] = -40.0  # its score lies 200 and more below the others
+    q = (_q(dtype, 1, 8).abs() + 0.5).to(dtype)
+    tables = torch.arange(8, dtype=torch.int32).view(1, 8).numpy()
+    _check(cuda_device, q, cache, tables, [128], _weighted)
+
+
+@pytest.mark.parametrize("dtype,ratio", [(torch.float16, 2.0 ** 26), (torch.bfloat16, 2.0 ** 26), (torch.bfloat16, 2.0 ** 60)])
+@pytest.mark.parametrize("lens", [[128, 33, 7], [300, 289, 300]])
+def test_groups_of_one_head_with_scales_far_apart(cuda_device, dtype, ratio, lens):
+    """The values of dims 64..127 are 2^26 or 2^60 times smaller than those of dims 0..63."""
+    Hkv = 2 if lens[0] < 300 else 640  # units of one tile, and of whole sequences
+    N = sum((n + 15) // 16 for n in lens)
+    cache = _cache(dtype, N, 1, Hkv, 4)
+    pairs = _pairs(cache)
+    high = 2.0 ** 12 if dtype == torch.float16 else 2.0 ** 20
+    pairs[..., 1, :, 0, :] *= high
+    pairs[..., 1, :, 1, :] *= high / ratio
+    _check(cuda_device, _q(dtype, 3, Hkv), cache, make_tables(lens, N, 3), lens, _weighted)
+
+
+@BOTH
+def test_outputs_carry_their_types_precision(cuda_device, dtype):
+    """Ordinary values, to the outputs' own rounding: few tokens, where each one's weight is large."""
+    lens = [1, 5, 17, 40, 100, 333]
+    N = sum((n + 15) // 16 for n in lens)
+    _check(cuda_device, _q(dtype, 6, 8), _cache(dtype, N, 1, 2, 4), make_tables(lens, N, 3), lens, _weighted)
