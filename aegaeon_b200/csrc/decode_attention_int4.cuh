@@ -8,18 +8,20 @@
 //       q . K = sum over groups of  s (q . c) + m (sum of q)
 //       sum_t p_t V_t = sum_t (p_t s_t) c_t + sum_t p_t m_t
 //     so the codes go to the tensor cores as they are, exactly, and scales and minima meet them
-//     in fp32. A key code becomes an fp16 number with one AND-OR: a nibble under the exponent of 64 reads
-//     as 64 + c, and the constant is taken out with the keys' minima (m - 64 s in place of m) in fp32.
-//   * S^T = K Q^T as in the 16-bit kernel (16 tokens x 8 heads of the group, m16n8k16), in fp16 for bf16
-//     queries too, scaled by a power of two. A lane's codes of a token are one 16-byte load; which dim
-//     sits where in the contraction is free as long as the query fragments follow.
+//     in fp32.
+//   * A code becomes a bf16 number with one AND: a nibble under a zero exponent is the subnormal c * 2^-133,
+//     or c * 2^-129 four bits further up (bf16's least normal binade has the spacing of its subnormals),
+//     exact on the tensor cores; the other operand carries a power of two that keeps the products within
+//     fp32's range. Beside fp16 queries, whose 11 bits bf16 does not hold, a key code is an fp16 number: a
+//     nibble under the exponent of 64 reads as 64 + c, and the constant is taken out with the keys' minima
+//     (m - 64 s in place of m) in fp32.
+//   * S^T = K Q^T as in the 16-bit kernel (16 tokens x 8 heads of the group, m16n8k16), in the queries' type.
+//     A lane's codes of a token are one 16-byte load; which dim sits where in the contraction is free as
+//     long as the query fragments follow.
 //   * O^T += V^T P^T in bf16: P * s, made in fp32, goes in as two bf16 parts (16 bits), each with the whole
-//     range of fp32's exponents, so that neither a token's nor a group's scale costs another one bits. A
-//     value code becomes a bf16 number with one AND: a nibble under a zero exponent is the subnormal
-//     c * 2^-133, or c * 2^-129 four bits further up (bf16's least normal binade has the spacing of its
-//     subnormals), exact on the tensor cores. P * s is held times a power of two that keeps the products
-//     away from fp32's ends. Token pairs share a 32-bit word, so that the transposed fragment comes out of
-//     the AND without a transposing load. sum p m is 4 FMAs a token and lane.
+//     range of fp32's exponents, so that neither a token's nor a group's scale costs another one bits.
+//     Token pairs share a 32-bit word, so that the transposed fragment comes out of the AND without a
+//     transposing load. sum p m is 4 FMAs a token and lane.
 //   * The tensor cores cut off what an addition pushes out of the accumulator, always downwards, so a sum
 //     of one sign drifts with its length. So odd tokens count from the top: with -P s they meet 15 - c (the
 //     AND's result with those four bits turned over, the same instruction), sum p (m + 15 s) in place of
@@ -72,7 +74,7 @@ __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t b
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
   return r;
 }
-// Nibbles k and k + 4 (k = 0..3) of a word as fp16 pairs, code + kBias, into a[k]. Under the exponent of
+// Nibbles k and k + 4 (k = 0..3) of a key word as fp16 pairs, code + kBias, into a[k]. Under the exponent of
 // 64 a nibble at mantissa bits 4..7 reads as 64 + c and one at bits 0..3 as 64 + c / 16, which one
 // packed FMA (16 x - 960, exact) turns into 64 + c: that leaves one shift for two nibbles, as the
 // integer pipe, half as wide as the FMA pipe, is the busier one.
@@ -89,15 +91,21 @@ __device__ __forceinline__ void code_pairs(uint32_t w, uint32_t (&a)[4]) {
   a[2] = up(and_or(t, 0x000f000fu, 0x54005400u));
   a[3] = and_or(t, 0x00f000f0u, 0x54005400u);
 }
-// The same nibbles of a value word as bf16 pairs: a[0], a[2] hold code * 2^-133, a[1], a[3] code * 2^-129, the
-// upper halves, which are odd tokens, 15 - code.
-__device__ __forceinline__ void value_codes(uint32_t w, uint32_t (&a)[4]) {
-  const uint32_t t = w >> 8;
-  a[0] = (w & 0x000f000fu) ^ 0x000f0000u;
-  a[1] = (w & 0x00f000f0u) ^ 0x00f00000u;
-  a[2] = (t & 0x000f000fu) ^ 0x000f0000u;
-  a[3] = (t & 0x00f000f0u) ^ 0x00f00000u;
+// The same nibbles as bf16 pairs: a[0], a[2] hold code * 2^-133, a[1], a[3] code * 2^-129; of values the upper
+// halves, which are odd tokens, 15 - code.
+template <bool kTurn>
+__device__ __forceinline__ void code_pairs_bf16(uint32_t w, uint32_t (&a)[4]) {
+  const uint32_t t = w >> 8, low = kTurn ? 0x000f0000u : 0u, high = kTurn ? 0x00f00000u : 0u;
+  a[0] = (w & 0x000f000fu) ^ low;
+  a[1] = (w & 0x00f000f0u) ^ high;
+  a[2] = (t & 0x000f000fu) ^ low;
+  a[3] = (t & 0x00f000f0u) ^ high;
 }
+// What bf16 queries, brought to 1 by a power of two, are held times (1 / 16 of it where they meet a[1], a[3]); the
+// products with the codes are then times 2^-13.
+constexpr float kQueryTop = 0x1p120f;
+// 2^n, -126 <= n <= 127.
+__device__ __forceinline__ float power_of_two(int n) { return __uint_as_float(static_cast<uint32_t>(n + 127) << 23); }
 // Two fp32 numbers as pairs of bf16: the upper 8 bits of each cut off, and the rest rounded to 8.
 __device__ __forceinline__ void split2(float y0, float y1, uint32_t& hi, uint32_t& lo) {
   const uint32_t b0 = __float_as_uint(y0), b1 = __float_as_uint(y1);
@@ -449,12 +457,15 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
     }
 
     // A negative scale goes into the sign of q, so that larger sums always mean larger scores. bf16
-    // queries go to fp16 exactly after a power of two of the head's own (elements below 2^-17 of the
-    // head's largest are rounded at 2^-24 of it), which returns with the scale of the scores.
+    // queries are brought to 1 by a power of two of the head's own, 2^-a, which returns with the scale of the
+    // scores: exactly, down to elements 2^-200 of the head's largest. Half of it, of the group's largest head,
+    // goes to the keys (2^(a / 2 - 8)): then large queries with small keys and small queries with large keys
+    // both leave the unscaled scores in fp32's range.
     const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
     uint32_t qf[NT][8][2];
     float qs[NT][2][2];  // [column][group]
     float sc[NT][2];     // scores to log2 units [column]
+    int e_top = 1;       // exponent of the group's largest finite |q|
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int head = nt * 8 + grp;
@@ -482,11 +493,12 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
         if constexpr (!std::is_same<T, __half>::value)
           for (int i = 0; i < 4; ++i) top = __vmaxu2(top, xw[w][i] & 0x7fff7fffu);
       }
-      float back = 1.f;
+      float back = 1.f, sum[2] = {0.f, 0.f};
       if constexpr (!std::is_same<T, __half>::value) {
         top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int e = static_cast<int>(max(top & 0xffffu, top >> 16) >> 7);  // exponent of the largest |q|
+        if (e < 255) e_top = max(e_top, e);
         const int ef = min(max(254 - e, 1), 253);
         const float to = __uint_as_float(static_cast<uint32_t>(ef) << 23);  // 2^(127 - e): |q| below 2
         back = __uint_as_float(static_cast<uint32_t>(254 - ef) << 23);
@@ -495,21 +507,25 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float2 f = unpack2<T>(xw[w][i]);
-            xw[w][i] = pack2<__half>(f.x * to, f.y * to);
+            const float x = f.x * to, y = f.y * to;
+            sum[w >> 1] += x + y;
+            xw[w][i] = pack2<T>(x * kQueryTop, y * (kQueryTop / 16.f));
+          }
+      } else {
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack2<T>(xw[w][i]);
+            sum[w >> 1] += f.x + f.y;
           }
       }
-      float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         qf[nt][2 * w][0] = __byte_perm(xw[w][0], xw[w][2], 0x5410);
         qf[nt][2 * w][1] = __byte_perm(xw[w][0], xw[w][2], 0x7632);
         qf[nt][2 * w + 1][0] = __byte_perm(xw[w][1], xw[w][3], 0x5410);
         qf[nt][2 * w + 1][1] = __byte_perm(xw[w][1], xw[w][3], 0x7632);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = unpack2<__half>(xw[w][i]);
-          sum[w >> 1] += f.x + f.y;
-        }
       }
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
@@ -518,11 +534,28 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
         qs[nt][0][g] = __shfl_sync(0xffffffffu, sum[g], 8 * quad);
         qs[nt][1][g] = __shfl_sync(0xffffffffu, sum[g], 8 * quad + 4);
       }
-      // Not 0, so that -infinity stays below all scores.
-      back = fmaxf(back * fabsf(p.scale_log2), 1e-37f);
       sc[nt][0] = __shfl_sync(0xffffffffu, back, 8 * quad);
       sc[nt][1] = __shfl_sync(0xffffffffu, back, 8 * quad + 4);
     }
+    float key_unit = 1.f;  // times the keys' scales
+    if constexpr (!std::is_same<T, __half>::value) {
+      e_top = __reduce_max_sync(0xffffffffu, e_top);
+      const int w = ((e_top - 127) >> 1) - 8;
+      key_unit = power_of_two(w + 13);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          sc[nt][i] *= power_of_two(-w);
+          qs[nt][i][0] *= power_of_two(w);
+          qs[nt][i][1] *= power_of_two(w);
+        }
+    }
+    // Not 0, so that -infinity stays below all scores, nor infinite, so that the largest keeps its weight.
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sc[nt][i] = fminf(fmaxf(sc[nt][i] * fabsf(p.scale_log2), 1e-37f), 3e38f);
     // The slot is free once every lane's values have arrived: the vote stored before the arrival needs
     // them all.
     if (!first) {
@@ -574,17 +607,29 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
 #pragma unroll
         for (int w = 2 * g; w < 2 * g + 2; ++w) {
           uint32_t lo[4], hi[4];
-          code_pairs(kw0[w], lo);
-          code_pairs(kw1[w], hi);
+          if constexpr (std::is_same<T, __half>::value) {
+            code_pairs(kw0[w], lo);
+            code_pairs(kw1[w], hi);
+          } else {
+            code_pairs_bf16<false>(kw0[w], lo);
+            code_pairs_bf16<false>(kw1[w], hi);
+          }
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const uint32_t a[4] = {lo[2 * u], hi[2 * u], lo[2 * u + 1], hi[2 * u + 1]};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_free<__half>(s[nt], a, qf[nt][2 * w + u][0], qf[nt][2 * w + u][1]);
+            for (int nt = 0; nt < NT; ++nt) mma_free<T>(s[nt], a, qf[nt][2 * w + u][0], qf[nt][2 * w + u][1]);
           }
         }
-        const float2 f0 = unpack2<T>(g == 0 ? kp0.x : kp0.y), f1 = unpack2<T>(g == 0 ? kp1.x : kp1.y);
-        const float b0 = fmaf(-kBias, f0.x, f0.y), b1 = fmaf(-kBias, f1.x, f1.y);
+        float2 f0 = unpack2<T>(g == 0 ? kp0.x : kp0.y), f1 = unpack2<T>(g == 0 ? kp1.x : kp1.y);
+        float b0 = f0.y, b1 = f1.y;
+        if constexpr (std::is_same<T, __half>::value) {
+          b0 = fmaf(-kBias, f0.x, b0);
+          b1 = fmaf(-kBias, f1.x, b1);
+        } else {
+          f0.x *= key_unit;
+          f1.x *= key_unit;
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -702,8 +747,8 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         uint32_t lo[4], hi[4];
-        value_codes(vw0[w], lo);
-        value_codes(vw1[w], hi);
+        code_pairs_bf16<true>(vw0[w], lo);
+        code_pairs_bf16<true>(vw1[w], hi);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t a[4] = {lo[2 * j], lo[2 * j + 1], hi[2 * j], hi[2 * j + 1]};

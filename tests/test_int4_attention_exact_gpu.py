@@ -1,6 +1,6 @@
 """Decode attention over a 4-bit cache whose values lie far apart, against the oracle in 64 bits: poisoned groups
 beside finite ones, scores too large for a difference of rounded products, tokens and groups whose scales differ
-by many powers of two.
+by many powers of two, query elements far below the head's largest.
 
 Tolerance (``_weighted``), from the exact weights w, scales s, minima m and values V of each token, for a
 sequence of n tokens (t tiles of 16):
@@ -31,7 +31,7 @@ def _pairs(cache):
 
 
 def _weighted(want, q, cache, layer, tables, lens, scale):
-    """The tolerance above, per output element. Keys' codes count with an offset of 64."""
+    """The tolerance above, per output element. In fp16 keys' codes count with an offset of 64."""
     B, Hq, _ = q.shape
     Hkv = cache.size(2)
     out = torch.empty_like(want)
@@ -44,7 +44,8 @@ def _weighted(want, q, cache, layer, tables, lens, scale):
         qg = q[b].double().view(Hkv, -1, 128)
         w = torch.softmax(torch.einsum("hgd,htd->hgt", qg, k) * scale, -1)
         sk, mk = (pairs[:, 0, :, :, i].repeat_interleave(64, -1) for i in (0, 1))  # Hkv, n, 128
-        terms = torch.einsum("hgd,htd->hgt", qg.abs(), 2 * 79 * sk + mk.abs())  # 64 + c, and 64 s beside m
+        size = 2 * 79 * sk + mk.abs() if q.dtype == torch.float16 else (k - mk).abs() + mk.abs()  # 64 + c, 64 s beside m
+        terms = torch.einsum("hgd,htd->hgt", qg.abs(), size)
         delta = (16 * 2.0 ** -22 + 2.0 ** -23) * terms.amax(-1) * abs(scale) * 1.5  # Hkv, G, in log2 units
         sv, mv = (pairs[:, 1, :, :, i].repeat_interleave(64, -1).nan_to_num() for i in (0, 1))
         ws = torch.einsum("hgt,htd->hgd", w, sv)
@@ -148,3 +149,30 @@ def test_outputs_carry_their_types_precision(cuda_device, dtype):
     lens = [1, 5, 17, 40, 100, 333]
     N = sum((n + 15) // 16 for n in lens)
     _check(cuda_device, _q(dtype, 6, 8), _cache(dtype, N, 1, 2, 4), make_tables(lens, N, 3), lens, _weighted)
+
+
+def test_small_elements_of_a_bf16_query_count_in_full(cuda_device):
+    """Dim 0 holds the query's largest element and the keys' zeros; the scores come from elements 2^-20 times
+    as large and keys of up to 10^6."""
+    dtype, n = torch.bfloat16, 60
+    cache = _cache(dtype, 4, 1, 1, 9)
+    raw = cache.view(torch.uint8).view(4, 1, 1, 2304)
+    raw[..., torch.arange(16) * 64] &= 0xf0  # key dim 0: code 0
+    pairs = _pairs(cache)
+    g = torch.Generator().manual_seed(5)
+    pairs[:, :, :, 0, :, :, 0] = (1e5 * (0.5 + torch.rand(4, 1, 1, 16, 2, generator=g))).to(dtype)
+    pairs[:, :, :, 0, :, :, 1] = 0
+    q = (torch.randn(1, 8, 128, generator=g) * 2.0 ** -20).to(dtype)
+    q[..., 0] = 1.0
+    _check(cuda_device, q, cache, torch.arange(4, dtype=torch.int32).view(1, 4).numpy(), [n], _weighted)
+
+
+@pytest.mark.parametrize("size", [1e-38, 1e-30, 1e30, 2e38])
+def test_bf16_queries_of_any_size(cuda_device, size):
+    """Scores of ordinary size from queries near either end of bf16's range; the keys' scales make up for it."""
+    dtype, lens = torch.bfloat16, [70, 16, 1, 300]
+    cache = _cache(dtype, 27, 1, 2, 9)
+    pairs = _pairs(cache)
+    pairs[:, :, :, 0] = (pairs[:, :, :, 0].double() / size).clamp(-3e38, 3e38).to(dtype)
+    q = (_q(dtype, 4, 8).double().clamp(-1.6, 1.6) * size).to(dtype)
+    _check(cuda_device, q, cache, make_tables(lens, 27, 3), lens, _weighted)
