@@ -143,6 +143,9 @@ fork_plan_kernel(const PoolParams p, const int64_t* src, const int64_t* dst, int
           if (!valid_id(tail, p.num_blocks)) {
             e.z = -1;
             report(AEG_DEVERR_BLOCK_ID_RANGE);
+          } else if (p.ref_counts[tail] <= 0) {  // free: this call may give it out while it is copied
+            e.z = -1;
+            report(AEG_DEVERR_POOL_ENTRY);
           }
         }
       } else {

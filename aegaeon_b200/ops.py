@@ -807,7 +807,7 @@ def fork_blocks(kv_cache: torch.Tensor, ref_counts: torch.Tensor, block_tables: 
     on the current stream, without reading anything back. Returns int32 ``[n]``: the block each fork
     took, or -1. Refused entries leave their row empty and raise a device error
     (``read_device_errors``): a row out of range, a target row that is not empty or named before, a
-    pool with no free block left.
+    last block that is free itself, a pool with no free block left.
     """
     index, N, width, rows = _check_shared(ref_counts, block_tables, seq_lens)
     nbytes = _check_pool(kv_cache, index, N)

@@ -446,10 +446,10 @@ AEG_API int aeg_rotary_multi_axis(void* q_out, int64_t q_out_stride, void* k_out
  * writing, is copied whole (block_bytes) into a free block. new_blocks[i] receives that block's id,
  * or -1. An entry is refused (row untouched, new_blocks[i] = -1, AEG_DEVERR_POOL_ENTRY) when a row
  * is outside the table, the source's length is outside it, the target row is not empty or an earlier
- * entry names it; AEG_DEVERR_BLOCK_ID_RANGE instead when the block to copy is outside the pool, and
- * AEG_DEVERR_POOL_EMPTY when no free block is left (later entries that need none still proceed).
- * Sources are read as they were before the call; their blocks must be live (sharing a free one raises
- * AEG_DEVERR_POOL_ENTRY, and the call may have given it out). */
+ * entry names it, or the block to copy is free; AEG_DEVERR_BLOCK_ID_RANGE instead when the block to
+ * copy is outside the pool, and AEG_DEVERR_POOL_EMPTY when no free block is left (later entries that
+ * need none still proceed). Sources are read as they were before the call; the blocks they share must
+ * be live (a free one raises AEG_DEVERR_POOL_ENTRY, except where the call has given it out). */
 AEG_API size_t aeg_fork_blocks_workspace_size(int64_t n);
 AEG_API int aeg_fork_blocks(void* pool, size_t block_bytes, int64_t num_blocks, int32_t* ref_counts,
                             int32_t* block_tables, int table_stride, int rows, int32_t* seq_lens,

@@ -164,7 +164,7 @@ class Pool:
         self.width = len(self.tables[0]) if self.tables else 0
 
     def fork(self, src, dst):
-        before = list(self.lens)
+        before, counts = list(self.lens), list(self.counts)
         taken, new, errors = set(), [], set()
         free = [b for b, c in enumerate(self.counts) if c == 0]
         copies = []
@@ -176,6 +176,9 @@ class Pool:
             n = (before[s] + 15) // 16
             if before[s] % 16 and not 0 <= self.tables[s][n - 1] < len(self.counts):
                 errors.add("id")
+                continue
+            if before[s] % 16 and counts[self.tables[s][n - 1]] <= 0:
+                errors.add("entry")
                 continue
             if d in taken:
                 errors.add("entry")

@@ -225,3 +225,16 @@ def test_a_captured_beam_step_replays(cuda_device):
         want, _ = b.o.fork(step, list(range(3, 9)))
         assert new.tolist() == want
         b.check()
+
+
+def test_copying_a_free_last_block_is_refused(cuda_device):
+    """A row whose partly filled last block has no references: the lowest free block, which another entry takes."""
+    b = Both(cuda_device, 8, 6, 2)
+    b.fill([0, 1], [20, 5])
+    tail = b.o.tables[0][1]
+    b.o.counts[tail] = 0
+    for block in range(tail):  # below it nothing is free
+        b.o.counts[block] = max(b.o.counts[block], 1)
+    b.sync_in()
+    b.fork([0, 1, 0, 1], [2, 3, 4, 4])
+    assert b.o.lens == [20, 5, 0, 5, 5, 0] and b.o.tables[3][0] == tail
