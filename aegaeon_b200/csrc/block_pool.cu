@@ -61,6 +61,15 @@ __device__ __forceinline__ int cta_scan(int v, int* s_warp, int& total) {
 }
 static_assert(kPlanThreads == 1024, "cta_scan sums 32 warps");
 
+__device__ __forceinline__ int ld_relaxed(const int* p) {
+  int v;
+  asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_relaxed(int* p, int v) {
+  asm volatile("st.relaxed.gpu.global.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+
 __device__ __forceinline__ bool valid_id(int64_t id, int64_t n) { return id >= 0 && id < n; }
 
 // The share of CTA-wide work (item) of copying one block: segment `seg` of src -> dst.
@@ -362,11 +371,11 @@ __global__ void __launch_bounds__(kCopyThreads) compact_apply_kernel(const PoolP
   pdl_enter();
   const int cap = p.table_stride * kBlockTokens;
   const int moves = ws.moves[0];
-  // Rows read remap while moving blocks' entries go from a place in the list to the id it stands for:
-  // either says the same.
+  // Rows read remap while moving blocks' entries go from a place in the list to the id it stands for: either
+  // says the same, and relaxed accesses see one of them whole.
   for (int r = blockIdx.x * kCopyThreads + threadIdx.x; r < moves; r += gridDim.x * kCopyThreads) {
     const int to = ws.list[r], from = ws.list[moves + r];
-    out.remap[from] = to;
+    st_relaxed(&out.remap[from], to);
     out.ref_counts[to] = p.ref_counts[from];
   }
   for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
@@ -380,7 +389,7 @@ __global__ void __launch_bounds__(kCopyThreads) compact_apply_kernel(const PoolP
     for (int j = threadIdx.x; j < p.table_stride; j += kCopyThreads) {
       int id = p.tables[base + j];
       if (j < nb) {
-        int to = valid_id(id, p.num_blocks) ? out.remap[id] : -1;
+        int to = valid_id(id, p.num_blocks) ? ld_relaxed(&out.remap[id]) : -1;
         if (to < -1) to = ws.list[-2 - to - moves];
         if (to >= 0) id = to;
         else report(AEG_DEVERR_BLOCK_ID_RANGE);
