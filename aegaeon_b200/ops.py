@@ -68,9 +68,20 @@ def _token_rows(t: torch.Tensor, name: str, what: str) -> torch.Size:
     shape = t.shape
     if len(shape) == 3:
         stride = t.stride()
-        if stride[2] == 1 and stride[1] == shape[2]:
+        if stride[2] == 1 and (stride[1] == shape[2] or shape[1] == 1):
             return shape
     raise ValueError(f"{name} must be {what} with contiguous heads")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements between the tokens of a ``_token_rows`` tensor; of a single token, whose stride means nothing,
+    the row's length."""
+    return t.stride(0) if t.size(0) != 1 else t.size(1) * t.size(2)
+
+
+def _table_stride(t: torch.Tensor) -> int:
+    """Entries between the rows of a block table; of a single row, its width."""
+    return t.stride(0) if t.size(0) != 1 else t.size(1)
 
 
 def _require_cuda(t: torch.Tensor, name: str) -> None:
@@ -619,7 +630,7 @@ def _int4_move(fn, what: str, key: torch.Tensor | None, value: torch.Tensor | No
             raise ValueError(f"kv_cache holds {Hkv} KV heads, not {heads}")
         if not (index == key.get_device() == value.get_device()):
             _on_devices(index, dict(key=key, value=value))
-        k_stride, v_stride = key.stride(0), value.stride(0)
+        k_stride, v_stride = _row_stride(key), _row_stride(value)
     if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (T,):
         raise ValueError("slot_mapping must be int64 [T]")
     slot_mapping = slot_mapping.contiguous()
@@ -706,8 +717,10 @@ def rotary_multi_axis(query: torch.Tensor, key: torch.Tensor, positions: torch.T
     if not usual:
         positions, inv_freq = _check_rotary(query, key, positions, inv_freq, axes, half)
         (T, Hq, D), Hkv = query.shape, key.size(1)
-        q_stride, k_stride, axis_stride = query.stride(0), key.stride(0), positions.stride(0)
+        q_stride, k_stride, axis_stride = _row_stride(query), _row_stride(key), positions.stride(0)
         dtype, index = query.dtype, query.get_device()
+    elif T == 1:  # a single token's stride means nothing
+        q_stride, k_stride = Hq * D, Hkv * D
     if query_out is None:
         query_out = torch.empty_like(query) if query.is_contiguous() else query.new_empty(query.shape)
     else:
@@ -716,8 +729,8 @@ def rotary_multi_axis(query: torch.Tensor, key: torch.Tensor, positions: torch.T
         key_out = torch.empty_like(key) if key.is_contiguous() else key.new_empty(key.shape)
     else:
         _check_rotary_out(index, key_out, key, "key_out")
-    _launch(index, "rotary_multi_axis", lib.aeg_rotary_multi_axis, query_out.data_ptr(), query_out.stride(0),
-            key_out.data_ptr(), key_out.stride(0), query.data_ptr(), q_stride, key.data_ptr(), k_stride,
+    _launch(index, "rotary_multi_axis", lib.aeg_rotary_multi_axis, query_out.data_ptr(), _row_stride(query_out),
+            key_out.data_ptr(), _row_stride(key_out), query.data_ptr(), q_stride, key.data_ptr(), k_stride,
             positions.data_ptr(), axis_stride, axes, inv_freq.data_ptr(), axis_of, half, float(scaling), T, Hq, Hkv, D,
             _DTYPES[dtype])
     return query_out, key_out
@@ -752,7 +765,7 @@ def _check_rotary_out(index: int, out: torch.Tensor, src: torch.Tensor, name: st
     shape = _token_rows(out, name, "its input's shape")
     if shape != src.shape or out.dtype != src.dtype:
         raise ValueError(f"{name} must match its input's shape and dtype")
-    if out.data_ptr() == src.data_ptr() and out.stride(0) != src.stride(0):
+    if out.data_ptr() == src.data_ptr() and _row_stride(out) != _row_stride(src):
         raise ValueError(f"{name} shares its input's memory with another stride")
     _on_device(index, out, name)
 
@@ -922,7 +935,7 @@ class DecodePlan:
             block_tables = block_tables.contiguous()
         int4 = self.cache == "int4"
         _launch(index, "decode_plan_int4" if int4 else "decode_plan", lib.aeg_decode_plan_int4 if int4 else lib.aeg_decode_plan,
-                self.workspace.data_ptr(), self.workspace.numel(), block_tables.data_ptr(), block_tables.stride(0),
+                self.workspace.data_ptr(), self.workspace.numel(), block_tables.data_ptr(), _table_stride(block_tables),
                 seq_lens.data_ptr(), self.batch, self.num_q_heads, self.num_kv_heads, self.head_dim)
         self.table_width = block_tables.size(1)
         self.seq_lens = seq_lens
@@ -1131,8 +1144,10 @@ def paged_attention_decode_int4(out: torch.Tensor, query: torch.Tensor, kv_cache
         if plan is None:  # an empty batch
             return
         (B, Hq, D), (N, L, Hkv, tile) = query.shape, kv_cache.shape
-        q_stride, out_stride, t_stride = query.stride(0), out.stride(0), block_tables.stride(0)
+        q_stride, out_stride, t_stride = _row_stride(query), _row_stride(out), _table_stride(block_tables)
         dtype, index = query.dtype, query.get_device()
+    elif B == 1:  # a single row's stride means nothing
+        q_stride, out_stride, t_stride = Hq * D, Hq * D, block_tables.size(1)
     ws = plan.workspace
     head = Hkv * INT4_TILE
     _launch(index, "paged_attention_decode_int4", lib.aeg_paged_attn_decode_int4, out.data_ptr(), out_stride,
