@@ -956,7 +956,8 @@ class DecodePlan:
                 cache: str = "auto") -> bool:
         tables, lens = self.block_tables, self.seq_lens
         return ((self.batch, self.num_q_heads, self.num_kv_heads, self.head_dim, self.cache) == (B, Hq, Hkv, D, cache)
-                and tables is not None and (tables is block_table or tables.data_ptr() == block_table.data_ptr())
+                and tables is not None and (tables is block_table or (tables.data_ptr() == block_table.data_ptr()
+                                                                      and _table_stride(tables) == _table_stride(block_table)))
                 and (lens is seq_lens or lens.data_ptr() == seq_lens.data_ptr())
                 and self.table_width == block_table.size(1))
 

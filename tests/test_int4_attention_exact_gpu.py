@@ -176,3 +176,19 @@ def test_bf16_queries_of_any_size(cuda_device, size):
     pairs[:, :, :, 0] = (pairs[:, :, :, 0].double() / size).clamp(-3e38, 3e38).to(dtype)
     q = (_q(dtype, 4, 8).double().clamp(-1.6, 1.6) * size).to(dtype)
     _check(cuda_device, q, cache, make_tables(lens, 27, 3), lens, _weighted)
+
+
+def test_a_plan_for_rows_laid_out_otherwise_is_refused(cuda_device):
+    """Tables that begin at the same address and are as wide, their rows further apart: other blocks."""
+    wide = torch.arange(16, dtype=torch.int32, device=cuda_device).view(2, 8)
+    near, far = wide.flatten()[:8].view(2, 4), wide[:, :4]
+    assert near.data_ptr() == far.data_ptr() and near.shape == far.shape
+    lens = torch.tensor([60, 64], dtype=torch.int32, device=cuda_device)
+    cache, q = _cache(torch.float16, 16, 1, 2, 3).to(cuda_device), _q(torch.float16, 2, 4).to(cuda_device)
+    kv = torch.zeros(16, 1, 2, 16, 2, 128, dtype=torch.float16, device=cuda_device)
+    for kind, call, pool in (("int4", ops.paged_attention_decode_int4, cache), ("auto", ops.paged_attention_decode, kv)):
+        plan = ops.DecodePlan(2, 4, 2, 128, cuda_device, cache=kind).plan(lens, near)
+        call(torch.empty_like(q), q, pool, 0, near, lens, SCALE, plan=plan)
+        call(torch.empty_like(q), q, pool, 0, wide.flatten()[:8].view(2, 4), lens, SCALE, plan=plan)
+        with pytest.raises(ValueError, match="plan"):
+            call(torch.empty_like(q), q, pool, 0, far, lens, SCALE, plan=plan)
