@@ -69,7 +69,8 @@ constexpr int kBlockTokens = 16;
 constexpr int kMaxWarps = 4096;         // worker warps of one launch the workspace is sized for
 constexpr int kPlanThreads = 256;
 constexpr int kUnitCost = 2;           // plan cost of starting a pair, in blocks (query load, epilogue)
-constexpr int kUnitCostInt4 = 4;       // the same over a 4-bit cache (64 sequences 10.3 us a layer, 11.0 at 2)
+constexpr int kUnitCostInt4 = 4;       // the same over a 4-bit cache (at 2: 64 chat sequences 10.9 us a layer, 10.3 at
+                                       // 4; 256 ragged 33.1, 32.7; 2 long 29.6, 29.3; 16 x 40/40 heads 77.0, 77.2)
 constexpr int kPlanLongUnits = 4;       // a pair with more units has them written by the whole plan CTA
 constexpr int kPlanLongPairs = 512;     // capacity of the plan's list of such pairs
 constexpr int kPlanCachedSeqs = 4096;   // sequences whose block counts the plan keeps in smem

@@ -31,20 +31,23 @@
 //   * One warp of the CTA requests the tiles of all others, a lane for each, so that walking the units
 //     and the block table costs the computing warps neither instructions nor registers.
 //
-// What bounds it, per layer inside a graph of layers (and the 16-bit kernel on the same lengths):
-//   4 sequences of 17..300 tokens, 28/4 heads fp16       8.3 us (7.1)   a chain of round trips
-//   64 of lognormal(5.5, 1) tokens, 28/4 heads fp16     10.3 us (13.0)
-//   256 of lognormal(6, 1) tokens, 32/4 heads bf16      33.1 us (58.0)  2.5 TB/s of K/V
-//   2 of 40,001..65,535 tokens, 32/4 heads bf16         27.6 us (46.7)
-//   16 of 2048..4096 tokens, 40/40 heads fp16           76.9 us (177)   3.8 TB/s
-// Streaming alone (nothing computed) takes 60 us of the last one, computing alone about as long as both
-// together: at 4.5 bits an element the work per byte is 3.6 times that of the 16-bit kernel, ~330
-// instructions a tile at half the issue rate (three warps a scheduler, 168 registers each). 15 workers of
-// 128 registers, 7 of 255, two tiles at a time in a worker, the next tile's scores ahead of this one's
-// products, 16 % fewer integer instructions: each within 5 % or slower. Workers that issue their own
-// copies, from a queue of addresses that the spare warp fills: 94 us for the last case, 38 for the third.
-// Start, split merge and the slowest SM take 8 to 14 us of a launch; the next layer's start overlaps most
-// of the first.
+// What it takes, per layer inside a graph of layers (the 16-bit kernel on the same lengths), and with the layer's
+// cache write before each attention, as a decode step has it (the 16-bit kernels likewise):
+//   4 sequences of 17..300 tokens, 28/4 heads fp16       7.6 us (6.9)    9.5 us (7.9)
+//   64 of lognormal(5.5, 1) tokens, 28/4 heads fp16     10.5 us (12.3)  13.7 us (13.7)
+//   256 of lognormal(6, 1) tokens, 32/4 heads bf16      33.7 us (55.6)  38.4 us (57.0)  2.5 TB/s of K/V
+//   2 of 40,001..65,535 tokens, 32/4 heads bf16         27.7 us (48.3)  29.2 us (49.8)
+//   16 of 2048..4096 tokens, 40/40 heads fp16           79.0 us (178)   84.3 us (182)   3.7 TB/s
+// What bounds it: walking the units, requesting nothing and computing nothing, start and merge included, took
+// 20.5 us of the fourth, 23.4 of the third and 37.2 of the last; requesting the tiles without computing 25.7,
+// 29.3 and 60.5. So the requesting warp's loop, one 2304-byte tile a step for each worker, uses up most of the
+// time the memory would need (85 clocks a tile and SM, of 100 for its bytes). Beside it the work per byte is
+// 3.6 times that of the 16-bit kernel, ~350 instructions a tile at half the issue rate (three warps a
+// scheduler, 168 registers each). 15 workers of 128 registers, 7 of 255, two tiles at a time in a worker,
+// the next tile's scores ahead of this one's products, 16 % fewer integer instructions: each within 5 % or
+// slower. Workers that issue their own copies, from a queue of addresses that the spare warp fills, took
+// 94 us for the last case, 38 for the third. P * scale in one fp16 number, of 11 bits under one power of two
+// for both groups, took 1 to 3 % less, and gave wrong values where scales lie far apart.
 
 template <int NT>
 struct Int4Smem {

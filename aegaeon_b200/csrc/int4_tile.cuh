@@ -151,8 +151,8 @@ __device__ __noinline__ uint2 int4_quantise_any(uint4 raw, float lo, float hi) {
 // Codes of a lane's 8 dims and its group's pair: {codes, dim n's at bits 4 n; scale | minimum << 16}. The
 // 8 lanes of a group are consecutive; the whole warp calls this together.
 //
-// Where no element but 0 is below 2^(p - 23) of the span (p: T's significant bits), every x - minimum is
-// a multiple of 2^-23 of the span or more. Then differences are exact in fp32, a quotient that is no tie
+// Where no element is below 2^(p - 23) of the span (p: T's significant bits; an exact 0 is taken for one, too),
+// every x - minimum is a multiple of 2^-23 of the span or more. Then differences are exact in fp32, a quotient that is no tie
 // differs from one by more than fp32's rounding, and a correctly rounded quotient gives the right code:
 // that is a product and two FMAs (Markstein's division with the rounded reciprocal), and adding 1.5 * 2^23
 // rounds it to a whole number, ties to even, with the code in the low bits. fp16 has no bits below 2^-24,

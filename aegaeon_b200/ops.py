@@ -1121,7 +1121,7 @@ def paged_attention_decode_int4(out: torch.Tensor, query: torch.Tensor, kv_cache
     Arguments as for ``paged_attention_decode``; ``plan`` is a ``DecodePlan(..., cache="int4")`` built
     for these tables and lengths. ``prefetch=True`` promises that the kernel launched just before on
     this stream writes neither this layer's blocks nor the block tables (so not right after the
-    layer's ``reshape_and_cache_int4``).
+    layer's ``reshape_and_cache_int4``); no kernel of this library further back is passed.
     """
     # A decode loop makes this call for every layer of every step, so its usual form is recognised in one
     # expression; anything else is checked piece by piece (and refused, or brought into that form).

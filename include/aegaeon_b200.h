@@ -396,9 +396,9 @@ AEG_API int aeg_gather_cache_int4(void* key, void* value, int64_t key_stride, in
                                   const int64_t* slot_mapping, int64_t T, int Hkv, int D, int dtype,
                                   void* stream);
 
-/* aeg_paged_attn_decode over a 4-bit cache: the same result for the values the cache holds (their
- * products and sums in fp32, the output rounded to `dtype` once; a row that reads back as NaN gives
- * NaN). The workspace is planned by aeg_decode_plan_int4 (same size and arguments as aeg_decode_plan;
+/* aeg_paged_attn_decode over a 4-bit cache: the same result for the values the cache holds (products and
+ * sums in fp32, a token's weight times its scale carried with 16 bits, the output rounded to `dtype` once; a
+ * group that reads back as NaN gives NaN in its 64 dims). The workspace is planned by aeg_decode_plan_int4 (same size and arguments as aeg_decode_plan;
  * a plan of the other kind raises AEG_DEVERR_PLAN_MISMATCH). A block id outside the pool raises
  * AEG_DEVERR_BLOCK_ID_RANGE and its tokens are left out. flags: 0 or AEG_DECODE_PREFETCH. D = 128,
  * Hq / Hkv <= 16, `kv_cache` 16-byte aligned, `scale` finite. */
