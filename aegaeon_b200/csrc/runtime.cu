@@ -2,7 +2,6 @@
 // sticky device error word reader.
 #include "aeg_common.cuh"
 
-#include <atomic>
 #include <mutex>
 #include <vector>
 
@@ -37,35 +36,53 @@ int num_sms() {
   return cache[dev];
 }
 
-// Per device the stream whose last noted launch is an attention; one at a time, so that another stream's
-// attention makes this one's writes start their successors later, never sooner.
+// Per device the stream, and the capture on it (0: none), whose last noted launch is an attention; one at a
+// time, so that another stream's attention makes this one's writes start their successors later, never sooner.
 namespace {
 constexpr int kTailDevices = 64;
 struct Tail {
-  std::atomic<bool> any{false};
-  std::atomic<cudaStream_t> stream{nullptr};
+  bool any = false;
+  cudaStream_t stream = nullptr;
+  unsigned long long capture = 0;
 };
-Tail* tail() {
-  static Tail t[kTailDevices];
+std::mutex g_tail_mu;
+Tail g_tail[kTailDevices];
+
+// The current device's entry and the capture on `s`; false where either cannot be told.
+bool find_tail(cudaStream_t s, Tail** t, unsigned long long* capture) {
   int dev = 0;
-  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kTailDevices ? &t[dev] : nullptr;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kTailDevices ||
+      cudaStreamGetCaptureInfo(s, &status, &id) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  *t = &g_tail[dev];
+  *capture = status == cudaStreamCaptureStatusNone ? 0 : id;
+  return true;
 }
 }  // namespace
 
 bool follows_attention(cudaStream_t s) {
-  const Tail* t = tail();
-  return t != nullptr && t->any.load() && t->stream.load() == s;
+  Tail* t = nullptr;
+  unsigned long long capture = 0;
+  if (!find_tail(s, &t, &capture)) return false;
+  std::lock_guard<std::mutex> lock(g_tail_mu);
+  return t->any && t->stream == s && t->capture == capture;
 }
 
 void note_launch(cudaStream_t s, bool attention) {
-  Tail* t = tail();
-  if (t == nullptr) return;
-  if (attention) {
-    t->any.store(false);  // no moment in which another stream passes for this one
-    t->stream.store(s);
-    t->any.store(true);
-  } else if (t->stream.load() == s) {
-    t->any.store(false);
+  Tail* t = nullptr;
+  unsigned long long capture = 0;
+  const bool known = find_tail(s, &t, &capture);
+  std::lock_guard<std::mutex> lock(g_tail_mu);
+  if (!known) {
+    for (Tail& x : g_tail) x.any = false;
+  } else if (attention) {
+    *t = Tail{true, s, capture};
+  } else if (t->stream == s && t->capture == capture) {
+    t->any = false;
   }
 }
 
