@@ -192,3 +192,57 @@ def test_a_plan_for_rows_laid_out_otherwise_is_refused(cuda_device):
         call(torch.empty_like(q), q, pool, 0, wide.flatten()[:8].view(2, 4), lens, SCALE, plan=plan)
         with pytest.raises(ValueError, match="plan"):
             call(torch.empty_like(q), q, pool, 0, far, lens, SCALE, plan=plan)
+
+
+# ---- wide groups, shared workspaces -----------------------------------------------------------------
+
+
+@BOTH
+@pytest.mark.parametrize("G", [9, 16])
+def test_groups_of_more_than_eight_heads(cuda_device, dtype, G):
+    """Two column tiles: ordinary values to the outputs' precision, scales 2^26 apart between the groups, and a
+    poisoned group in units of 19 tiles (more pairs than the 1036 workers)."""
+    lens = [1, 17, 333]
+    N = sum((n + 15) // 16 for n in lens)
+    cache, tables = _cache(dtype, N, 1, 2, 4), make_tables(lens, N, 3)
+    _check(cuda_device, _q(dtype, 3, 2 * G), cache, tables, lens, _weighted)
+    pairs = _pairs(cache)
+    pairs[..., 1, :, 0, :] *= 2.0 ** 12
+    pairs[..., 1, :, 1, :] *= 2.0 ** -14
+    _check(cuda_device, _q(dtype, 3, 2 * G), cache, tables, lens, _weighted)
+    lens, Hkv = [300, 289, 300], 400
+    cache = _cache(dtype, 19, 1, Hkv, 6)
+    _pairs(cache)[0, 0, ::4, 1, 0, 0] = float("nan")
+    _pairs(cache)[9, 0, 1::4, 1, 0, 1] = float("nan")
+    tables = torch.arange(19, dtype=torch.int32).repeat(3, 1).numpy()
+    _check(cuda_device, _q(dtype, 3, Hkv * G), cache, tables, lens, _weighted)
+
+
+def test_two_captured_graphs_share_a_workspace(cuda_device):
+    """One plan's step in two graphs, each with its own queries and layers, replayed in any order."""
+    dtype, N, lens = torch.float16, 260, [3000, 40, 0, 177, 16]
+    cache, tables = _cache(dtype, N, 3, 2, 12).to(cuda_device), torch.as_tensor(make_tables(lens, N, 5)).to(cuda_device)
+    sl = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    plan = ops.DecodePlan(5, 14, 2, 128, cuda_device, cache="int4")
+    qs = [_q(dtype, 5, 14, i).to(cuda_device) for i in range(2)]
+    outs = [[torch.empty_like(qs[0]) for _ in range(3)] for _ in range(2)]
+
+    def step(i):
+        plan.plan(sl, tables)
+        for layer in range(3):
+            ops.paged_attention_decode_int4(outs[i][layer], qs[i], cache, layer, tables, sl, SCALE, plan=plan, prefetch=layer > 0)
+
+    want, graphs = [], []
+    for i in range(2):
+        step(i)
+        torch.cuda.synchronize()
+        want.append([o.clone() for o in outs[i]])
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            step(i)
+    for i in (0, 1, 1, 0, 0, 1):
+        for o in outs[i]:
+            o.fill_(7)
+        graphs[i].replay()
+        assert all(torch.equal(a, b) for a, b in zip(outs[i], want[i]))
+    assert ops.read_device_errors(cuda_device) == 0

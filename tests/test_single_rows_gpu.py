@@ -1,4 +1,4 @@
-"""One token, one sequence, one head: dimensions of size 1, whose strides mean nothing. A single token laid out
+"""One token, one sequence, one head or no key head: dimensions of size 1, whose strides mean nothing. A single token laid out
 heads first is contiguous, whatever its first stride says."""
 import math
 
@@ -74,3 +74,15 @@ def test_one_head(cuda_device):
     for cache, x in zip(caches, (k, _odd_strides(k))):
         ops.reshape_and_cache_int4(x, x, cache, 0, pos + 3)
     assert torch.equal(caches[0].view(torch.int16), caches[1].view(torch.int16))
+
+
+def test_queries_without_keys_and_positions_below_zero(cuda_device):
+    g = torch.Generator(cuda_device).manual_seed(4)
+    q = torch.randn(9, 4, 128, generator=g, device=cuda_device).half()
+    pos, inv = torch.arange(-4, 5, device=cuda_device) * 1000, torch.rand(64, generator=g, device=cuda_device)
+    want = ops.rotary_multi_axis(q, q, pos, inv, (64,))[0]
+    got, none = ops.rotary_multi_axis(q, q[:, :0], pos, inv, (64,))
+    assert torch.equal(got, want) and none.shape == (9, 0, 128)
+    back, _ = ops.rotary_multi_axis(want, want, -pos, inv, (64,))
+    # two roundings to fp16 of numbers that a rotation may mix with a partner of up to 5
+    assert ((back.double() - q.double()).abs() <= 2 * 2.0 ** -11 * (q.double().abs() + 5)).all()
