@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(Int4Smem<NT>::kThreads, 1) decode_attn_int4_ke
 
     // A negative scale goes into the sign of q, so that larger sums always mean larger scores. bf16
     // queries are brought to 1 by a power of two of the head's own, 2^-a, which returns with the scale of the
-    // scores: exactly, down to elements 2^-200 of the head's largest. Half of it, of the group's largest head,
+    // scores: exactly, down to elements 2^-110 of the head's largest. Half of it, of the group's largest head,
     // goes to the keys (2^(a / 2 - 8)): then large queries with small keys and small queries with large keys
     // both leave the unscaled scores in fp32's range.
     const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;

@@ -106,8 +106,8 @@ def test_scores_of_any_size_pick_the_largest(cuda_device, dtype, size, sign):
         q = torch.full((1, 8, 128), size, dtype=dtype)
         got = _run(cuda_device, q, cache, 0, torch.arange(16, dtype=torch.int32).view(1, 16).numpy(), [n])
         want = ref.values(cache[:, 0])[1][best // 16, :, best % 16].repeat_interleave(4, 0)
-        # P * s with 11 bits times codes up to 8 off the middle; the scale is below 0.35, the minimum below 8
-        bound = want.abs() * torch.finfo(dtype).eps / 2 + 2.0 ** -11 * 8 * 0.35 + 2.0 ** -20 * 8
+        # P * s with 16 bits times codes up to 15; the scale is below 0.35, the minimum below 8
+        bound = want.abs() * torch.finfo(dtype).eps / 2 + 2.0 ** -16 * 15 * 0.35 + 2.0 ** -20 * 8
         assert ((got[0].double() - want).abs() <= bound).all()
 
 
